@@ -1,0 +1,68 @@
+// Matrix products grouped by expert over rows of ragged counts: parameters and
+// launchers shared by the kernel's translation units and the torch bindings.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+namespace abacus {
+namespace ragged {
+
+constexpr int kMaxExperts = 256;
+
+enum Epilogue : int { kStore = 0, kSwiGLU = 1, kSwiGLUBwd = 2 };
+
+// What a launch computes, over sorted rows r of expert e = [offsets[e], offsets[e + 1]):
+//  rows, store:      out0[r] = sum over segments s of a[s][r] B[s][e]
+//  rows, SwiGLU:     out0 = a B[0], out1 = a B[1], out2 = silu(out0) * out1
+//  rows, SwiGLU bwd: dh = a B[0]; out0 = dh u sig (1 + g (1 - sig)), out1 = dh g sig  (g = in0, u = in1)
+//  weights:          out_o[e] = sum over r of a[r]^T b[o][r]
+// Rows at or after offsets[experts] get zeros.
+struct alignas(64) Params {
+  CUtensorMap a[2];
+  CUtensorMap b[2];
+  const int* offsets;
+  int experts;
+  int rows;      // all sorted rows, owned or not
+  int k;         // rows: length of a contraction segment
+  int segments;  // rows: 1 or 2
+  int m;         // weights: rows of an output matrix
+  int n;         // columns of an output (hidden units for SwiGLU)
+  int n_tiles;   // column tiles of one output
+  int outputs;   // weights: 1 or 2
+  void* out[3];
+  const void* in[2];
+  int wide;      // rows of out and in can move in 16-byte units
+  int* status;
+};
+
+struct Shape {
+  int planes;   // bf16 parts of an operand: 1 (bf16), 2 or 3 (fp32)
+  bool pair;    // two CTAs on one 256 x 256 tile, or one CTA on a 128 x 128 tile
+  bool weights; // which of the two kinds of product
+  bool b_mn;    // rows: B is stored (k, n) rather than (n, k)
+  Epilogue epilogue;
+};
+
+// Tile of a shape.
+constexpr int tile_rows(bool pair) { return pair ? 256 : 128; }
+constexpr int tile_cols(bool pair) { return pair ? 256 : 128; }
+
+// Launches with at most `units` output tiles to do; cudaErrorInvalidValue for a combination that is not built.
+cudaError_t launch(const Params& p, const Shape& s, long long units, int sms, cudaStream_t stream);
+template <int PLANES, bool PAIR>
+cudaError_t launch_shape(const Params& p, const Shape& s, long long units, int sms, cudaStream_t stream);
+
+// bf16 parts of a (batch, rows, cols) tensor of any strides, in `planes` consecutive (batch, rows, ld) arrays; columns
+// cols .. ld - 1 are zeros. planes == 1 takes bf16 (a copy), else fp32.
+struct StageParams {
+  const void* src;
+  bool src_bf16;
+  long long stride_batch, stride_row, stride_col;
+  long long batch, rows, cols, ld;
+  int planes;
+  void* dst;
+};
+cudaError_t launch_stage(const StageParams& p, int sms, cudaStream_t stream);
+
+}  // namespace ragged
+}  // namespace abacus

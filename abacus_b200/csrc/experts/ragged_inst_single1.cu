@@ -1,0 +1,7 @@
+#include "ragged_kernel.cuh"
+
+namespace abacus {
+namespace ragged {
+template cudaError_t launch_shape<1, false>(const Params&, const Shape&, long long, int, cudaStream_t);
+}  // namespace ragged
+}  // namespace abacus

@@ -1,0 +1,664 @@
+// The kernel behind the ragged expert products (see ragged.h for the sums).
+//
+// bf16 operands run as they are. An fp32 operand arrives as 2 or 3 bf16 parts
+// (planes) x = h + m + l, each the rounded remainder of the ones before, 8
+// significant bits apiece: three hold all 24 bits of x. Their products of
+// order up to 2^-16 (h h, h m, m h, m m, h l, l h) give x y to 2^-25; with two
+// planes h h, h m and m h give it to 2^-16 (the framework's tf32 mode has
+// 2^-11). A bf16 product costs half a tf32 one, so six of them cost what the
+// three of the 3xTF32 kernels do, with no conversion inside this kernel: the
+// planes are laid out by one pass over each operand before it.
+//
+// Accumulation: the tensor core adds in fp32 but truncates. With one plane a
+// tile's whole sum stays in tensor memory (the outputs are rounded to 8 bits).
+// With several planes each 64 elements of the contraction go into a fresh
+// accumulator, small products first, and the epilogue warps add it to their
+// registers rounding to nearest, so the error is that of an fp32 sum.
+//
+// Roles of a CTA (384 threads): warp 0 loads tiles by TMA, warp 1 issues the
+// MMAs, warp 2 clears the rows of a tile that belong to the next expert (the
+// contraction of `weights` runs over rows, so they would be added; both
+// operands are cleared, so that nothing infinite meets a zero), warps 4-11 are
+// the epilogue. In a pair (cta_group::2) each CTA holds 128 of the tile's 256
+// rows and half of B's 256 columns: 64 KB from L2 per 64-deep step for both,
+// where two single CTAs of 128 x 256 would read 96 KB. Persistent CTAs walk
+// the tiles; accumulators are double buffered, so a tile's epilogue runs under
+// the next tile's MMAs.
+#pragma once
+#include <cuda_bf16.h>
+#include <type_traits>
+#include "../common/host.h"
+#include "../common/sm100.cuh"
+#include "ragged.h"
+
+namespace abacus {
+namespace ragged {
+
+constexpr int kDepth = 64;        // contraction elements of a stage: 128 bytes of bf16, one swizzle span
+constexpr int kThreads = 384;
+constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
+constexpr int kStageOutBytes = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes
+
+template <int PLANES, bool PAIR>
+struct Config {
+  static constexpr int kBN = tile_cols(PAIR);
+  static constexpr int kLocalCols = PAIR ? kBN / 2 : kBN;  // columns of B in this CTA
+  static constexpr int kABytes = 128 * kDepth * 2;
+  static constexpr int kBBytes = kLocalCols * kDepth * 2;
+  static constexpr int kStageBytes = PLANES * (kABytes + kBBytes);
+  static constexpr int kStages = 6 / PLANES;  // 192 KB of stages
+  static constexpr uint32_t kTmemCols = 2 * kBN;
+  static constexpr int kTableBytes = (kMaxExperts + 2) * 4;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kStageOutBytes + kTableBytes;
+};
+
+__device__ __forceinline__ uint64_t desc_mnmajor_bf16(uint32_t saddr) {
+  // 64 columns (128 bytes) x 64 rows a chunk: chunks 8 KB apart, 8-row groups 1 KB apart.
+  return make_smem_desc(saddr, kDepth * 128, 1024, kLayoutSw128);
+}
+
+__host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, bool a_mn_major, bool b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10)  // D fp32, A and B bf16
+         | ((a_mn_major ? 1u : 0u) << 15) | ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (PAIR) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// Tile load that counts its bytes on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_expect_cluster(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+
+__device__ __forceinline__ void arrive_release_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// 16-byte unit `unit` of row `row` of an epilogue warp's staging rows, so that both a column of units over eight rows
+// and a row of units touch every bank once.
+template <int UNITS>
+__device__ __forceinline__ uint32_t unit_at(int row, int unit) {
+  return UNITS == 8 ? row * 128 + ((unit ^ (row & 7)) << 4) : row * 64 + ((unit ^ ((row >> 1) & 3)) << 4);
+}
+
+template <class Out>
+struct OutTraits;
+template <>
+struct OutTraits<float> {
+  static constexpr int kPerUnit = 4;
+  __device__ static float zero() { return 0.f; }
+  __device__ static uint4 pack(const float* v) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
+  __device__ static void unpack(uint4 u, float* v) {
+    v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
+  }
+};
+template <>
+struct OutTraits<__nv_bfloat16> {
+  static constexpr int kPerUnit = 8;
+  __device__ static __nv_bfloat16 zero() { return __float2bfloat16_rn(0.f); }
+  __device__ static uint4 pack(const float* v) {
+    uint4 u;
+    uint32_t* w = &u.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    return u;
+  }
+  __device__ static void unpack(uint4 u, float* v) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+
+// 32 columns of a warp's 32 rows, a row a lane, between registers and global memory through the warp's staging rows,
+// so that global accesses run along rows. `rows` of them exist, and columns below `cols`.
+template <class Out>
+struct Rows32 {
+  using Traits = OutTraits<Out>;
+  static constexpr int kUnits = 32 / Traits::kPerUnit;  // 16-byte units of 32 columns
+  static constexpr int kRowsAtOnce = 32 / kUnits;
+
+  __device__ static void store(uint8_t* staging, int lane, Out* base, long long ld, int rows, int col0, int cols, bool wide,
+                               const float* v) {
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u)
+      *reinterpret_cast<uint4*>(staging + unit_at<kUnits>(lane, u)) = Traits::pack(v + u * Traits::kPerUnit);
+    __syncwarp();
+    if (wide) {
+      const int unit = lane % kUnits;
+      const int col = col0 + unit * Traits::kPerUnit;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int r = i * kRowsAtOnce + lane / kUnits;
+        if (r < rows && col < cols)
+          *reinterpret_cast<uint4*>(base + r * ld + col) = *reinterpret_cast<const uint4*>(staging + unit_at<kUnits>(r, unit));
+      }
+    } else {
+      const int unit = lane / Traits::kPerUnit, in = lane % Traits::kPerUnit;
+      if (col0 + lane < cols) {
+        for (int r = 0; r < rows; ++r)
+          base[r * ld + col0 + lane] = reinterpret_cast<const Out*>(staging + unit_at<kUnits>(r, unit))[in];
+      }
+    }
+  }
+
+  __device__ static void load(uint8_t* staging, int lane, const Out* base, long long ld, int rows, int col0, int cols,
+                              bool wide, float* v) {
+    __syncwarp();
+    if (wide) {
+      const int unit = lane % kUnits;
+      const int col = col0 + unit * Traits::kPerUnit;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int r = i * kRowsAtOnce + lane / kUnits;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < rows && col < cols) x = *reinterpret_cast<const uint4*>(base + r * ld + col);
+        *reinterpret_cast<uint4*>(staging + unit_at<kUnits>(r, unit)) = x;
+      }
+    } else {
+      const int unit = lane / Traits::kPerUnit, in = lane % Traits::kPerUnit;
+      for (int r = 0; r < 32; ++r)
+        reinterpret_cast<Out*>(staging + unit_at<kUnits>(r, unit))[in] =
+            r < rows && col0 + lane < cols ? base[r * ld + col0 + lane] : Traits::zero();
+    }
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u)
+      Traits::unpack(*reinterpret_cast<const uint4*>(staging + unit_at<kUnits>(lane, u)), v + u * Traits::kPerUnit);
+  }
+};
+
+struct Tile {
+  int expert;     // == experts: rows that nobody owns
+  int row0;       // rows: first sorted row of this CTA's 128; weights: first output row of them
+  int row_end;    // end of the rows that exist
+  int n0;         // first output column
+  int output;     // weights: which output
+  int steps;      // stages of the contraction
+  int k_row0;     // weights: first sorted row of the contraction
+  int k_rows;     // weights: their number
+};
+
+template <int PLANES, bool PAIR, bool WEIGHTS, bool B_MN, Epilogue EPI>
+__global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_constant__ Params p) {
+  using Cfg = Config<PLANES, PAIR>;
+  using Out = typename std::conditional<PLANES == 1, __nv_bfloat16, float>::type;
+  constexpr int kStages = Cfg::kStages;
+  constexpr bool A_MN = WEIGHTS;
+  constexpr int kTileM = tile_rows(PAIR);
+  constexpr int kTileCols = EPI == kSwiGLU ? Cfg::kBN / 2 : Cfg::kBN;  // output columns of a tile
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_bar[kStages], empty_bar[kStages], tail_bar[kStages];
+  __shared__ uint64_t accum_full[2], accum_empty[2];
+  __shared__ uint32_t tmem_base_slot;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const bool leader = rank == 0;
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  uint8_t* staging = smem + kStages * Cfg::kStageBytes;
+  int* tile_start = reinterpret_cast<int*>(staging + kEpiWarps * kStageOutBytes);
+  auto leader_addr = [&](uint64_t* bar) { return PAIR ? mapa_shared(smem_u32(bar), 0) : smem_u32(bar); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_bar[s], PAIR ? 2 : 1);  // one arrival for each CTA's share of the stage
+      mbar_init(&empty_bar[s], 1);
+      mbar_init(&tail_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accum_full[b], 1);
+      mbar_init(&accum_empty[b], PAIR ? 2 * kEpiWarps : kEpiWarps);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&p.a[0]);
+    tma_prefetch_desc(&p.b[0]);
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(&tmem_base_slot, Cfg::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&tmem_base_slot, Cfg::kTmemCols);
+      tmem_relinquish();
+    }
+  }
+  // Offsets are the caller's device data: whatever they hold, every range used is inside [0, rows].
+  auto offset_at = [&](int e) { return e == 0 ? 0 : min(max(p.offsets[e], 0), p.rows); };
+  if (!WEIGHTS && warp == 3) {
+    // Row tiles before each expert; the rows after the last one's are expert number `experts`.
+    int carry = 0;
+    for (int e0 = 0; e0 <= p.experts; e0 += 32) {
+      const int e = e0 + lane;
+      int tiles = 0;
+      if (e <= p.experts) {
+        const int begin = offset_at(e), end = e == p.experts ? p.rows : offset_at(e + 1);
+        tiles = (max(end - begin, 0) + kTileM - 1) / kTileM;
+        if (end < begin && blockIdx.x == 0) atomicCAS(p.status, kStatusOk, kStatusBadArgs);
+      }
+      int sum = tiles;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += o;
+      }
+      if (e <= p.experts) tile_start[e] = carry + sum - tiles;
+      carry += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) tile_start[p.experts + 1] = carry;
+  }
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync_all();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_slot;
+
+  // ---------------------------------------------------------------- schedule
+  const int m_tiles = WEIGHTS ? (p.m + kTileM - 1) / kTileM : 0;
+  const long long units = WEIGHTS ? static_cast<long long>(p.experts) * m_tiles * p.n_tiles * p.outputs
+                                  : static_cast<long long>(tile_start[p.experts + 1]) * p.n_tiles;
+  const long long first_unit = PAIR ? blockIdx.x / 2 : blockIdx.x;
+  const long long unit_step = PAIR ? gridDim.x / 2 : gridDim.x;
+  const int steps_per_segment = WEIGHTS ? 0 : (p.k + kDepth - 1) / kDepth;
+  // `e` is where the caller's walk stands (units only grow along it).
+  auto tile_at = [&](long long unit, int& e) {
+    Tile t;
+    if constexpr (WEIGHTS) {
+      const int per_expert = m_tiles * p.n_tiles * p.outputs;
+      t.expert = static_cast<int>(unit / per_expert);
+      const int in = static_cast<int>(unit - static_cast<long long>(t.expert) * per_expert);
+      const int column = in / m_tiles;
+      t.row0 = (in % m_tiles) * kTileM + static_cast<int>(rank) * 128;
+      t.row_end = p.m;
+      t.output = column / p.n_tiles;
+      t.n0 = (column % p.n_tiles) * kTileCols;
+      t.k_row0 = offset_at(t.expert);
+      t.k_rows = max(offset_at(t.expert + 1) - t.k_row0, 0);
+      t.steps = (t.k_rows + kDepth - 1) / kDepth;
+    } else {
+      const int row_tile = static_cast<int>(unit / p.n_tiles);
+      while (tile_start[e + 1] <= row_tile) ++e;
+      t.expert = e;
+      t.row0 = offset_at(e) + (row_tile - tile_start[e]) * kTileM + static_cast<int>(rank) * 128;
+      t.row_end = e == p.experts ? p.rows : offset_at(e + 1);
+      t.n0 = static_cast<int>(unit - static_cast<long long>(row_tile) * p.n_tiles) * kTileCols;
+      t.output = 0;
+      t.k_row0 = t.k_rows = 0;
+      t.steps = e == p.experts ? 0 : p.segments * steps_per_segment;
+    }
+    return t;
+  };
+
+  if (warp == 0) {
+    // -------------------------------------------------------------- loads
+    if (elect_one_sync()) {
+      long long it = 0;
+      bool ok = true;
+      int e = 0;
+      for (long long unit = first_unit; unit < units && ok; unit += unit_step) {
+        const Tile t = tile_at(unit, e);
+        for (int step = 0; step < t.steps; ++step, ++it) {
+          const int s = static_cast<int>(it % kStages);
+          const long long use = it / kStages;
+          if (use > 0 && !mbar_wait(&empty_bar[s], (use - 1) & 1, p.status, kStatusTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          const bool tail = WEIGHTS && (step + 1) * kDepth > t.k_rows;
+          uint32_t bar;
+          if (tail) {
+            bar = smem_u32(&tail_bar[s]);
+            mbar_arrive_expect_tx(&tail_bar[s], Cfg::kStageBytes);
+          } else {
+            bar = leader_addr(&full_bar[s]);
+            if (PAIR) arrive_expect_cluster(bar, Cfg::kStageBytes);
+            else mbar_arrive_expect_tx(&full_bar[s], Cfg::kStageBytes);
+          }
+          auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, int z) {
+            if constexpr (PAIR) tma_load_3d_pair(smem_u32(dst), map, bar, x, y, z);
+            else tma_load_3d(dst, map, tail ? &tail_bar[s] : &full_bar[s], x, y, z);
+          };
+          const int segment = WEIGHTS ? 0 : step / max(steps_per_segment, 1);
+          const int k0 = WEIGHTS ? t.k_row0 + step * kDepth : (step - segment * steps_per_segment) * kDepth;
+#pragma unroll
+          for (int pl = 0; pl < PLANES; ++pl) {
+            uint8_t* a = smem + s * Cfg::kStageBytes + pl * Cfg::kABytes;
+            uint8_t* b = smem + s * Cfg::kStageBytes + PLANES * Cfg::kABytes + pl * Cfg::kBBytes;
+            if constexpr (A_MN) {
+              load(a, &p.a[0], t.row0, k0, pl);
+              load(a + Cfg::kABytes / 2, &p.a[0], t.row0 + 64, k0, pl);
+            } else {
+              load(a, &p.a[segment], k0, t.row0, pl);
+            }
+            const int z = WEIGHTS ? pl : pl * p.experts + t.expert;
+            if constexpr (EPI == kSwiGLU) {
+              // One half of the tile's columns of B are gate columns, the other half the same up columns.
+              if constexpr (PAIR) {
+#pragma unroll
+                for (int c = 0; c < Cfg::kLocalCols / 64; ++c)
+                  load(b + c * 8192, &p.b[rank], t.n0 + 64 * c, k0, z);
+              } else {
+                load(b, &p.b[0], t.n0, k0, z);
+                load(b + 8192, &p.b[1], t.n0, k0, z);
+              }
+            } else if constexpr (B_MN) {
+              const CUtensorMap* map = WEIGHTS ? &p.b[t.output] : &p.b[segment];
+#pragma unroll
+              for (int c = 0; c < Cfg::kLocalCols / 64; ++c)
+                load(b + c * 8192, map, t.n0 + static_cast<int>(rank) * Cfg::kLocalCols + 64 * c, k0, z);
+            } else {
+              load(b, &p.b[segment], k0, t.n0 + static_cast<int>(rank) * Cfg::kLocalCols, z);
+            }
+          }
+        }
+      }
+      // Leave only when every stage was read (and the leader's last commits have arrived here); after an error, when
+      // loads in flight have had time to land.
+      for (long long j = it > kStages ? it - kStages : 0; j < it; ++j)
+        if (!mbar_wait(&empty_bar[j % kStages], (j / kStages) & 1, nullptr, 0)) break;
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------------- MMAs
+    if (leader && elect_one_sync()) {
+      constexpr uint32_t idesc = idesc_bf16(kTileM, Cfg::kBN, A_MN, B_MN);
+      auto commit = [&](uint64_t* bar) {
+        if constexpr (PAIR) {
+          mma_commit_pair(smem_u32(bar));
+          mma_commit_pair(mapa_shared(smem_u32(bar), 1));
+        } else {
+          mma_commit(bar);
+        }
+      };
+      long long it = 0, acc = 0;  // stages and accumulators used so far
+      bool ok = true;
+      int e = 0;
+      for (long long unit = first_unit; unit < units && ok; unit += unit_step) {
+        const Tile t = tile_at(unit, e);
+        for (int step = 0; step < t.steps; ++step, ++it) {
+          const bool first = PLANES > 1 || step == 0;
+          const int buf = static_cast<int>(acc & 1);
+          if (first && acc >= 2 &&
+              !mbar_wait(&accum_empty[buf], ((acc >> 1) - 1) & 1, p.status, kStatusTimeoutAccum)) {
+            ok = false;
+            break;
+          }
+          const int s = static_cast<int>(it % kStages);
+          if (!mbar_wait(&full_bar[s], (it / kStages) & 1, p.status, kStatusTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d = tmem_base + static_cast<uint32_t>(buf * Cfg::kBN);
+          const uint32_t a0 = smem_u32(smem + s * Cfg::kStageBytes), b0 = a0 + PLANES * Cfg::kABytes;
+          auto product = [&](int pa, int pb, bool fresh) {
+#pragma unroll
+            for (int ks = 0; ks < kDepth / 16; ++ks) {
+              const uint32_t a = a0 + pa * Cfg::kABytes + (A_MN ? ks * 16 * 128 : ks * 32);
+              const uint32_t b = b0 + pb * Cfg::kBBytes + (B_MN ? ks * 16 * 128 : ks * 32);
+              mma_bf16<PAIR>(d, A_MN ? desc_mnmajor_bf16(a) : desc_kmajor_sw128(a),
+                             B_MN ? desc_mnmajor_bf16(b) : desc_kmajor_sw128(b), idesc, fresh && ks == 0 ? 0u : 1u);
+            }
+          };
+          if constexpr (PLANES == 3) {
+            product(2, 0, true);
+            product(0, 2, false);
+            product(1, 1, false);
+          }
+          if constexpr (PLANES >= 2) {
+            product(1, 0, PLANES == 2);
+            product(0, 1, false);
+          }
+          product(0, 0, PLANES == 1 && first);
+          commit(&empty_bar[s]);
+          if (PLANES > 1 || step + 1 == t.steps) {
+            commit(&accum_full[buf]);
+            ++acc;
+          }
+        }
+      }
+      for (long long j = it > kStages ? it - kStages : 0; j < it; ++j)
+        if (!mbar_wait(&empty_bar[j % kStages], (j / kStages) & 1, nullptr, 0)) break;
+    }
+  } else if (warp == 2) {
+    // -------------------------------------------------------------- rows of the next expert
+    if constexpr (WEIGHTS) {
+      long long it = 0;
+      uint32_t parity = 0;  // of each stage's tail barrier
+      int e = 0;
+      for (long long unit = first_unit; unit < units; unit += unit_step) {
+        const Tile t = tile_at(unit, e);
+        it += t.steps;
+        const int valid = t.k_rows % kDepth;
+        if (valid == 0) continue;  // no rows at all, or whole stages
+        const int s = static_cast<int>((it - 1) % kStages);
+        if (!mbar_wait_warp(&tail_bar[s], (parity >> s) & 1, p.status, kStatusTimeoutConvert)) break;
+        parity ^= 1u << s;
+        // All chunks of a stage are 64 rows of 128 bytes; swizzling stays inside a row.
+        uint8_t* stage = smem + s * Cfg::kStageBytes;
+        const int units16 = (kDepth - valid) * 8;
+        for (int chunk = 0; chunk < Cfg::kStageBytes / 8192; ++chunk)
+          for (int u = lane; u < units16; u += 32)
+            *reinterpret_cast<uint4*>(stage + chunk * 8192 + valid * 128 + u * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) arrive_release_cluster(leader_addr(&full_bar[s]));
+          else mbar_arrive(&full_bar[s]);
+        }
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    // -------------------------------------------------------------- epilogue
+    constexpr int kCols = Cfg::kBN / 2;  // columns of a thread: half a row of the tile
+    constexpr int kGroups = kCols / 32;
+    const int quarter = warp % 4, half = (warp - kEpiWarp0) / 4;
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint8_t* mine = staging + (warp - kEpiWarp0) * kStageOutBytes;
+    // Tensor-memory column of a thread's group: for SwiGLU its gate columns, then the same up columns.
+    auto tmem_col = [&](int g) {
+      if constexpr (EPI == kSwiGLU)
+        return (g < kGroups / 2 ? 0 : Cfg::kBN / 2) + half * (kCols / 2) + 32 * (g % (kGroups / 2));
+      else
+        return half * kCols + 32 * g;
+    };
+    long long acc_count = 0;
+    bool ok = true;
+    int e = 0;
+    for (long long unit = first_unit; unit < units && ok; unit += unit_step) {
+      const Tile t = tile_at(unit, e);
+      const int row0 = t.row0 + quarter * 32;
+      const int rows = min(max(t.row_end - row0, 0), 32);
+      float acc[PLANES > 1 ? kCols : 1];
+      int buf = 0;
+      if constexpr (PLANES > 1) {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+        for (int step = 0; step < t.steps && ok; ++step, ++acc_count) {
+          buf = static_cast<int>(acc_count & 1);
+          ok = mbar_wait_warp(&accum_full[buf], (acc_count >> 1) & 1, p.status, kStatusTimeoutAccum);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) {
+            uint32_t v[32];
+            tmem_ld32(taddr + buf * Cfg::kBN + tmem_col(g), v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[g * 32 + i] += __uint_as_float(v[i]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) mbar_arrive_cluster(leader_addr(&accum_empty[buf]));
+            else mbar_arrive(&accum_empty[buf]);
+          }
+        }
+      } else if (t.steps > 0) {
+        buf = static_cast<int>(acc_count & 1);
+        ok = mbar_wait_warp(&accum_full[buf], (acc_count >> 1) & 1, p.status, kStatusTimeoutAccum);
+        tc_fence_after();
+      }
+      if (!ok) break;
+      auto group = [&](int g, float (&v)[32]) {
+        if constexpr (PLANES > 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = acc[g * 32 + i];
+        } else if (t.steps > 0) {
+          uint32_t raw[32];
+          tmem_ld32(taddr + buf * Cfg::kBN + tmem_col(g), raw);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+        }
+      };
+      const long long ld = p.n;
+      const long long first = (WEIGHTS ? static_cast<long long>(t.expert) * p.m : 0) + row0;
+      auto out = [&](int o) { return static_cast<Out*>(p.out[o]) + first * ld; };
+      auto in = [&](int i) { return static_cast<const Out*>(p.in[i]) + first * ld; };
+      if constexpr (EPI == kStore) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float v[32];
+          group(g, v);
+          Rows32<Out>::store(mine, lane, out(t.output), ld, rows, t.n0 + half * kCols + 32 * g, p.n, p.wide, v);
+        }
+      } else if constexpr (EPI == kSwiGLU) {
+#pragma unroll
+        for (int g = 0; g < kGroups / 2; ++g) {
+          float gate[32], up[32];
+          group(g, gate);
+          group(g + kGroups / 2, up);
+          const int col = t.n0 + half * (kCols / 2) + 32 * g;
+          Rows32<Out>::store(mine, lane, out(0), ld, rows, col, p.n, p.wide, gate);
+          Rows32<Out>::store(mine, lane, out(1), ld, rows, col, p.n, p.wide, up);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) up[i] *= gate[i] / (1.f + __expf(-gate[i]));
+          Rows32<Out>::store(mine, lane, out(2), ld, rows, col, p.n, p.wide, up);
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float dh[32], gate[32], up[32];
+          group(g, dh);
+          const int col = t.n0 + half * kCols + 32 * g;
+          if (t.steps > 0) {
+            Rows32<Out>::load(mine, lane, in(0), ld, rows, col, p.n, p.wide, gate);
+            Rows32<Out>::load(mine, lane, in(1), ld, rows, col, p.n, p.wide, up);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float sig = 1.f / (1.f + __expf(-gate[i]));
+              const float d_up = dh[i] * gate[i] * sig;
+              dh[i] = dh[i] * up[i] * sig * (1.f + gate[i] * (1.f - sig));
+              up[i] = d_up;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) up[i] = 0.f;
+          }
+          Rows32<Out>::store(mine, lane, out(0), ld, rows, col, p.n, p.wide, dh);
+          Rows32<Out>::store(mine, lane, out(1), ld, rows, col, p.n, p.wide, up);
+        }
+      }
+      if (PLANES == 1 && t.steps > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster(leader_addr(&accum_empty[buf]));
+          else mbar_arrive(&accum_empty[buf]);
+        }
+        ++acc_count;
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync_all();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    else tmem_dealloc(tmem_base, Cfg::kTmemCols);
+  }
+}
+
+template <int PLANES, bool PAIR, bool WEIGHTS, bool B_MN, Epilogue EPI>
+cudaError_t launch_one(const Params& p, long long units, int sms, cudaStream_t stream) {
+  using Cfg = Config<PLANES, PAIR>;
+  const auto kernel = ragged_kernel<PLANES, PAIR, WEIGHTS, B_MN, EPI>;
+  static host::PerDeviceOnce once;
+  cudaError_t err = cudaSuccess;
+  once.run([&] { err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes); });
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  const long long at_once = PAIR ? sms / 2 : sms;
+  const long long grid = units < at_once ? units : at_once;
+  cfg.gridDim = dim3(static_cast<unsigned>((grid < 1 ? 1 : grid) * (PAIR ? 2 : 1)));
+  if (PAIR) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int PLANES, bool PAIR>
+cudaError_t launch_shape(const Params& p, const Shape& s, long long units, int sms, cudaStream_t stream) {
+  if (s.weights) return launch_one<PLANES, PAIR, true, true, kStore>(p, units, sms, stream);
+  if (s.epilogue == kStore) {
+    return s.b_mn ? launch_one<PLANES, PAIR, false, true, kStore>(p, units, sms, stream)
+                  : launch_one<PLANES, PAIR, false, false, kStore>(p, units, sms, stream);
+  }
+  if (s.epilogue == kSwiGLU && s.b_mn) return launch_one<PLANES, PAIR, false, true, kSwiGLU>(p, units, sms, stream);
+  if (s.epilogue == kSwiGLUBwd && !s.b_mn) return launch_one<PLANES, PAIR, false, false, kSwiGLUBwd>(p, units, sms, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace ragged
+}  // namespace abacus

@@ -1,0 +1,91 @@
+// Operands of the ragged products that TMA cannot read as they are: fp32 ones
+// (split into bf16 parts), and bf16 ones whose rows are not 16-byte aligned.
+// Bound by memory: 4 bytes read and 2 per plane written an element. A thread
+// makes 8 columns: two 16-byte loads where the layout allows, one 16-byte
+// store per plane.
+#include <cuda_bf16.h>
+#include "../common/sm100.cuh"
+#include "ragged.h"
+
+namespace abacus {
+namespace ragged {
+namespace {
+
+// x = h + m + l with each part the rounded remainder of those before. An
+// infinite or NaN x is h alone; a finite one too large to round up to bf16 is
+// cut instead, so that it stays finite.
+__device__ __forceinline__ void split(float x, int planes, __nv_bfloat16 (&part)[3]) {
+  const bool finite = isfinite(x);
+  float h = __bfloat162float(__float2bfloat16_rn(x));
+  if (finite && !isfinite(h)) h = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  part[0] = __float2bfloat16_rn(h);
+  const float r = finite ? x - h : 0.f;
+  const float m = __bfloat162float(__float2bfloat16_rn(r));
+  part[1] = __float2bfloat16_rn(m);
+  part[2] = __float2bfloat16_rn(r - m);
+}
+
+__global__ void __launch_bounds__(256) stage_kernel(const StageParams p, bool vec, long long groups) {
+  const long long per_row = p.ld / 8;
+  const long long plane = p.batch * p.rows * p.ld;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < groups;
+       i += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const long long row = i / per_row;  // of all batches
+    const long long c0 = (i - row * per_row) * 8;
+    const long long b = row / p.rows, r = row - b * p.rows;
+    const long long at = b * p.stride_batch + r * p.stride_row + c0 * p.stride_col;
+    __nv_bfloat16 out[3][8];
+    if (p.src_bf16) {
+      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.src) + at;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[0][j] = c0 + j < p.cols ? src[j * p.stride_col] : __float2bfloat16_rn(0.f);
+    } else {
+      const float* src = static_cast<const float*>(p.src) + at;
+      float x[8];
+      if (vec) {  // whole groups of 8 columns, 16-byte aligned
+        const float4 u = *reinterpret_cast<const float4*>(src), v = *reinterpret_cast<const float4*>(src + 4);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = c0 + j < p.cols ? src[j * p.stride_col] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        __nv_bfloat16 part[3];
+        split(x[j], p.planes, part);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) out[q][j] = part[q];
+      }
+    }
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.dst) + row * p.ld + c0;
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+      if (q < p.planes) *reinterpret_cast<uint4*>(dst + q * plane) = *reinterpret_cast<const uint4*>(out[q]);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_stage(const StageParams& p, int sms, cudaStream_t stream) {
+  const long long groups = p.batch * p.rows * (p.ld / 8);
+  if (groups == 0) return cudaSuccess;
+  const bool vec = !p.src_bf16 && p.stride_col == 1 && p.cols % 8 == 0 && p.stride_row % 4 == 0 &&
+                   p.stride_batch % 4 == 0 && reinterpret_cast<uintptr_t>(p.src) % 16 == 0;
+  const long long blocks = (groups + 255) / 256, most = static_cast<long long>(sms) * 32;
+  stage_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(p, vec, groups);
+  return cudaGetLastError();
+}
+
+cudaError_t launch(const Params& p, const Shape& s, long long units, int sms, cudaStream_t stream) {
+  if (s.planes == 1)
+    return s.pair ? launch_shape<1, true>(p, s, units, sms, stream) : launch_shape<1, false>(p, s, units, sms, stream);
+  if (s.planes == 2)
+    return s.pair ? launch_shape<2, true>(p, s, units, sms, stream) : launch_shape<2, false>(p, s, units, sms, stream);
+  if (s.planes == 3)
+    return s.pair ? launch_shape<3, true>(p, s, units, sms, stream) : launch_shape<3, false>(p, s, units, sms, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace ragged
+}  // namespace abacus
