@@ -89,13 +89,52 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* map, 
       : "memory");
 }
 
+// Relaxed: this arrival publishes no data of the thread (the copies count their own bytes), and a release at cluster
+// scope would wait for a memory barrier on every stage.
 __device__ __forceinline__ void arrive_expect_cluster(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
 }
 
 __device__ __forceinline__ void arrive_release_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Bounded wait. The common header's wait reads the nanosecond timer as soon as a barrier is not ready, which takes about
+// as long as a stage's MMAs; a wait of this kernel usually ends within a stage, so it polls a while before it starts the
+// clock.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* status, int code) {
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, status, code);
+}
+__device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity, status, code));
+}
+
+// Stage of a pipeline position and the parity of its use.
+template <int STAGES>
+struct Position {
+  int stage = 0;
+  uint32_t parity = 0;  // of the stage's current use
+  bool wrapped = false; // every stage was used before
+  __device__ void next() {
+    if (++stage == STAGES) {
+      stage = 0;
+      parity ^= 1u;
+      wrapped = true;
+    }
+  }
+};
+
+// Waits until the last use of every stage was read, after `at` positions were filled.
+template <int STAGES>
+__device__ __forceinline__ void drain(uint64_t* empty_bar, Position<STAGES> at) {
+  for (int s = 0; s < STAGES; ++s) {
+    const bool this_round = s < at.stage;
+    if (!this_round && !at.wrapped) continue;  // never used
+    if (!mbar_wait(&empty_bar[s], this_round ? at.parity : at.parity ^ 1u, nullptr, 0)) break;
+  }
 }
 
 // 16-byte unit `unit` of row `row` of an epilogue warp's staging rows, so that both a column of units over eight rows
@@ -328,18 +367,24 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
   if (warp == 0) {
     // -------------------------------------------------------------- loads
     if (elect_one_sync()) {
-      long long it = 0;
+      Position<kStages> at;
       bool ok = true;
       int e = 0;
       for (long long unit = first_unit; unit < units && ok; unit += unit_step) {
         const Tile t = tile_at(unit, e);
-        for (int step = 0; step < t.steps; ++step, ++it) {
-          const int s = static_cast<int>(it % kStages);
-          const long long use = it / kStages;
-          if (use > 0 && !mbar_wait(&empty_bar[s], (use - 1) & 1, p.status, kStatusTimeoutEmpty)) {
+        int segment = 0, k_next = WEIGHTS ? t.k_row0 : 0;
+        for (int step = 0; step < t.steps; ++step, at.next()) {
+          const int s = at.stage;
+          if (at.wrapped && !wait_bar(&empty_bar[s], at.parity ^ 1u, p.status, kStatusTimeoutEmpty)) {
             ok = false;
             break;
           }
+          if (!WEIGHTS && step == steps_per_segment) {
+            segment = 1;
+            k_next = 0;
+          }
+          const int k0 = k_next;
+          k_next += kDepth;
           const bool tail = WEIGHTS && (step + 1) * kDepth > t.k_rows;
           uint32_t bar;
           if (tail) {
@@ -354,8 +399,6 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
             if constexpr (PAIR) tma_load_3d_pair(smem_u32(dst), map, bar, x, y, z);
             else tma_load_3d(dst, map, tail ? &tail_bar[s] : &full_bar[s], x, y, z);
           };
-          const int segment = WEIGHTS ? 0 : step / max(steps_per_segment, 1);
-          const int k0 = WEIGHTS ? t.k_row0 + step * kDepth : (step - segment * steps_per_segment) * kDepth;
 #pragma unroll
           for (int pl = 0; pl < PLANES; ++pl) {
             uint8_t* a = smem + s * Cfg::kStageBytes + pl * Cfg::kABytes;
@@ -390,8 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       }
       // Leave only when every stage was read (and the leader's last commits have arrived here); after an error, when
       // loads in flight have had time to land.
-      for (long long j = it > kStages ? it - kStages : 0; j < it; ++j)
-        if (!mbar_wait(&empty_bar[j % kStages], (j / kStages) & 1, nullptr, 0)) break;
+      drain<kStages>(empty_bar, at);
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMAs
@@ -405,21 +447,21 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
           mma_commit(bar);
         }
       };
-      long long it = 0, acc = 0;  // stages and accumulators used so far
+      Position<kStages> at;
+      Position<2> acc;
       bool ok = true;
       int e = 0;
       for (long long unit = first_unit; unit < units && ok; unit += unit_step) {
         const Tile t = tile_at(unit, e);
-        for (int step = 0; step < t.steps; ++step, ++it) {
+        for (int step = 0; step < t.steps; ++step, at.next()) {
           const bool first = PLANES > 1 || step == 0;
-          const int buf = static_cast<int>(acc & 1);
-          if (first && acc >= 2 &&
-              !mbar_wait(&accum_empty[buf], ((acc >> 1) - 1) & 1, p.status, kStatusTimeoutAccum)) {
+          const int buf = acc.stage;
+          if (first && acc.wrapped && !wait_bar(&accum_empty[buf], acc.parity ^ 1u, p.status, kStatusTimeoutAccum)) {
             ok = false;
             break;
           }
-          const int s = static_cast<int>(it % kStages);
-          if (!mbar_wait(&full_bar[s], (it / kStages) & 1, p.status, kStatusTimeoutFull)) {
+          const int s = at.stage;
+          if (!wait_bar(&full_bar[s], at.parity, p.status, kStatusTimeoutFull)) {
             ok = false;
             break;
           }
@@ -448,12 +490,11 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
           commit(&empty_bar[s]);
           if (PLANES > 1 || step + 1 == t.steps) {
             commit(&accum_full[buf]);
-            ++acc;
+            acc.next();
           }
         }
       }
-      for (long long j = it > kStages ? it - kStages : 0; j < it; ++j)
-        if (!mbar_wait(&empty_bar[j % kStages], (j / kStages) & 1, nullptr, 0)) break;
+      drain<kStages>(empty_bar, at);
     }
   } else if (warp == 2) {
     // -------------------------------------------------------------- rows of the next expert
@@ -467,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
         const int valid = t.k_rows % kDepth;
         if (valid == 0) continue;  // no rows at all, or whole stages
         const int s = static_cast<int>((it - 1) % kStages);
-        if (!mbar_wait_warp(&tail_bar[s], (parity >> s) & 1, p.status, kStatusTimeoutConvert)) break;
+        if (!wait_bar_warp(&tail_bar[s], (parity >> s) & 1, p.status, kStatusTimeoutConvert)) break;
         parity ^= 1u << s;
         // All chunks of a stage are 64 rows of 128 bytes; swizzling stays inside a row.
         uint8_t* stage = smem + s * Cfg::kStageBytes;
@@ -497,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       else
         return half * kCols + 32 * g;
     };
-    long long acc_count = 0;
+    Position<2> at;
     bool ok = true;
     int e = 0;
     for (long long unit = first_unit; unit < units && ok; unit += unit_step) {
@@ -509,9 +550,9 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       if constexpr (PLANES > 1) {
 #pragma unroll
         for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
-        for (int step = 0; step < t.steps && ok; ++step, ++acc_count) {
-          buf = static_cast<int>(acc_count & 1);
-          ok = mbar_wait_warp(&accum_full[buf], (acc_count >> 1) & 1, p.status, kStatusTimeoutAccum);
+        for (int step = 0; step < t.steps && ok; ++step, at.next()) {
+          buf = at.stage;
+          ok = wait_bar_warp(&accum_full[buf], at.parity, p.status, kStatusTimeoutAccum);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -530,8 +571,8 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
           }
         }
       } else if (t.steps > 0) {
-        buf = static_cast<int>(acc_count & 1);
-        ok = mbar_wait_warp(&accum_full[buf], (acc_count >> 1) & 1, p.status, kStatusTimeoutAccum);
+        buf = at.stage;
+        ok = wait_bar_warp(&accum_full[buf], at.parity, p.status, kStatusTimeoutAccum);
         tc_fence_after();
       }
       if (!ok) break;
@@ -605,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
           if (PAIR) mbar_arrive_cluster(leader_addr(&accum_empty[buf]));
           else mbar_arrive(&accum_empty[buf]);
         }
-        ++acc_count;
+        at.next();
       }
     }
   }
