@@ -16,7 +16,9 @@ enum Epilogue : int { kStore = 0, kSwiGLU = 1, kSwiGLUBwd = 2 };
 //  rows, SwiGLU:     out0 = a B[0], out1 = a B[1], out2 = silu(out0) * out1
 //  rows, SwiGLU bwd: dh = a B[0]; out0 = dh u sig (1 + g (1 - sig)), out1 = dh g sig  (g = in0, u = in1)
 //  weights:          out_o[e] = sum over r of a[r]^T b[o][r]
-// Rows at or after offsets[experts] get zeros.
+// Rows at or after offsets[experts] get zeros. What the SwiGLU forms hand to the next product (its out2, its
+// backward's out0 and out1) is written as that product's operand, in bf16 planes; their rows and those of g and u are
+// padded to whole 16-byte units, which the other results (the caller's contiguous tensors) may not be.
 struct alignas(64) Params {
   CUtensorMap a[2];
   CUtensorMap b[2];
@@ -31,7 +33,10 @@ struct alignas(64) Params {
   int outputs;   // weights: 1 or 2
   void* out[3];
   const void* in[2];
-  int wide;      // rows of out and in can move in 16-byte units
+  long long ld[3];     // row stride of out, in elements
+  long long ld_in;     // of in
+  long long plane;     // distance of the planes of an operand that is written
+  int wide;            // rows of a plain result can move in 16-byte units
   int* status;
 };
 

@@ -68,6 +68,23 @@ void check_result(const torch::Tensor& t, const torch::Tensor& like, int64_t pla
               name, " must be a contiguous ", planes == 1 ? "bf16" : "fp32", " tensor of shape ", shape);
 }
 
+// Rows that a SwiGLU form keeps for itself: (rows, cols) with rows padded to 16 bytes.
+void check_kept(const torch::Tensor& t, const torch::Tensor& like, int64_t planes, int64_t rows, int64_t cols, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols &&
+                  t.scalar_type() == (planes == 1 ? torch::kBFloat16 : torch::kFloat32) && t.stride(1) == 1 &&
+                  t.stride(0) * t.element_size() % 16 == 0 && t.stride(0) >= (cols * t.element_size() + 15) / 16 * 16 / t.element_size() &&
+                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              name, " must have 16-byte aligned rows");
+}
+
+// An operand that a SwiGLU form writes: (planes, rows, cols) with padded rows.
+void check_written(const torch::Tensor& t, const torch::Tensor& like, int64_t planes, int64_t rows, int64_t cols, const char* name) {
+  check_operand(t, 3, name);
+  TORCH_CHECK(t.device() == like.device() && t.size(0) == planes && t.size(1) == rows && t.size(2) == cols &&
+                  t.stride(1) % 8 == 0 && t.stride(1) >= (cols + 7) / 8 * 8 && t.stride(0) == rows * t.stride(1),
+              name, " must be (planes, rows, columns) with padded rows");
+}
+
 bool wide(std::initializer_list<torch::Tensor> ts, int64_t n) {
   bool ok = true;
   for (const auto& t : ts)
@@ -169,6 +186,7 @@ void rows(std::vector<torch::Tensor> a, std::vector<torch::Tensor> b, torch::Ten
   p.n = static_cast<int>(n);
   p.n_tiles = tiles_of(n, tile_cols(shape.pair));
   p.out[0] = out.data_ptr();
+  p.ld[0] = n;
   p.wide = wide({out}, n);
   run(p, shape, out);
 }
@@ -182,7 +200,8 @@ void swiglu(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, torch::Te
     check_rows_and_matrices(x, w, p.experts, k, "the experts' matrices");
     TORCH_CHECK(w.size(2) == k && w.size(3) == n, "ragged SwiGLU shapes");
   }
-  for (const auto& t : {g, u, h}) check_result(t, x, planes, {s, n}, "gate, up and product");
+  for (const auto& t : {g, u}) check_kept(t, x, planes, s, n, "gate and up");
+  check_written(h, x, planes, s, n, "their product");
   if (s == 0 || n == 0) return;
   TORCH_CHECK(k > 0, "empty contraction");
   Shape shape = {static_cast<int>(planes), use_pair_rows(p), false, true, kSwiGLU};
@@ -195,7 +214,10 @@ void swiglu(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, torch::Te
   p.out[0] = g.data_ptr();
   p.out[1] = u.data_ptr();
   p.out[2] = h.data_ptr();
-  p.wide = wide({g, u, h}, n);
+  p.ld[0] = g.stride(0);
+  p.ld[1] = u.stride(0);
+  p.ld[2] = h.stride(1);
+  p.plane = h.stride(0);
   run(p, shape, x);
 }
 
@@ -206,7 +228,9 @@ void swiglu_bwd(torch::Tensor dy, torch::Tensor w_down, torch::Tensor offsets, t
   Params p = params_of(offsets, dy, s);
   check_rows_and_matrices(dy, w_down, p.experts, k, "the down matrices");
   TORCH_CHECK(w_down.size(2) == n && w_down.size(3) == k, "ragged SwiGLU backward shapes");
-  for (const auto& t : {g, u, dg, du}) check_result(t, dy, planes, {s, n}, "gate, up and their gradients");
+  for (const auto& t : {g, u}) check_kept(t, dy, planes, s, n, "gate and up");
+  for (const auto& t : {dg, du}) check_written(t, dy, planes, s, n, "the gradients of gate and up");
+  TORCH_CHECK(g.stride(0) == u.stride(0), "gate and up must have one row stride");
   if (s == 0 || n == 0) return;
   TORCH_CHECK(k > 0, "empty contraction");
   Shape shape = {static_cast<int>(planes), use_pair_rows(p), false, false, kSwiGLUBwd};
@@ -219,7 +243,11 @@ void swiglu_bwd(torch::Tensor dy, torch::Tensor w_down, torch::Tensor offsets, t
   p.in[1] = u.data_ptr();
   p.out[0] = dg.data_ptr();
   p.out[1] = du.data_ptr();
-  p.wide = wide({g, u, dg, du}, n);
+  p.ld_in = g.stride(0);
+  p.ld[0] = dg.stride(1);
+  p.ld[1] = du.stride(1);
+  p.plane = dg.stride(0);
+  TORCH_CHECK(du.stride(0) == dg.stride(0), "the gradients of gate and up must be laid out alike");
   run(p, shape, dy);
 }
 
@@ -251,6 +279,7 @@ void weights(torch::Tensor x, std::vector<torch::Tensor> dy, torch::Tensor offse
   p.m = static_cast<int>(m);
   p.n = static_cast<int>(n);
   p.n_tiles = tiles_of(n, tile_cols(shape.pair));
+  p.ld[0] = n;
   p.wide = wide({dw[0], dw.back()}, n);
   run(p, shape, x);
 }

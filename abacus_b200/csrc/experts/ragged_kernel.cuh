@@ -30,6 +30,7 @@
 #include "../common/host.h"
 #include "../common/sm100.cuh"
 #include "ragged.h"
+#include "split.cuh"
 
 namespace abacus {
 namespace ragged {
@@ -49,6 +50,10 @@ struct Config {
   static constexpr int kStages = 6 / PLANES;  // 192 KB of stages
   static constexpr uint32_t kTmemCols = 2 * kBN;
   static constexpr int kTableBytes = (kMaxExperts + 2) * 4;
+  // Register split with several planes, whose epilogue threads hold half a row of fp32 sums: 128 x 72 + 256 x 216 is
+  // what 384 threads are launched with (168 each).
+  static constexpr uint32_t kRegsControl = 72, kRegsEpilogue = 216;
+  static_assert(128 * kRegsControl + 256 * kRegsEpilogue <= kThreads * 168, "register split above the launch's total");
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kStageOutBytes + kTableBytes;
 };
 
@@ -137,11 +142,13 @@ __device__ __forceinline__ void drain(uint64_t* empty_bar, Position<STAGES> at) 
   }
 }
 
-// 16-byte unit `unit` of row `row` of an epilogue warp's staging rows, so that both a column of units over eight rows
-// and a row of units touch every bank once.
+// Byte offset of 16-byte unit `unit` of row `row` in an epilogue warp's staging rows of UNITS units, such that both a
+// column of units over eight rows and eight units along rows touch every bank once.
 template <int UNITS>
 __device__ __forceinline__ uint32_t unit_at(int row, int unit) {
-  return UNITS == 8 ? row * 128 + ((unit ^ (row & 7)) << 4) : row * 64 + ((unit ^ ((row >> 1) & 3)) << 4);
+  static_assert(UNITS == 8 || UNITS == 4 || UNITS == 2, "32 to 128 bytes a row");
+  constexpr int kShift = UNITS == 8 ? 0 : UNITS == 4 ? 1 : 2;
+  return row * UNITS * 16 + ((unit ^ ((row >> kShift) & (UNITS - 1))) << 4);
 }
 
 template <class Out>
@@ -149,7 +156,6 @@ struct OutTraits;
 template <>
 struct OutTraits<float> {
   static constexpr int kPerUnit = 4;
-  __device__ static float zero() { return 0.f; }
   __device__ static uint4 pack(const float* v) {
     return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
   }
@@ -160,7 +166,6 @@ struct OutTraits<float> {
 template <>
 struct OutTraits<__nv_bfloat16> {
   static constexpr int kPerUnit = 8;
-  __device__ static __nv_bfloat16 zero() { return __float2bfloat16_rn(0.f); }
   __device__ static uint4 pack(const float* v) {
     uint4 u;
     uint32_t* w = &u.x;
@@ -181,8 +186,8 @@ struct OutTraits<__nv_bfloat16> {
   }
 };
 
-// 32 columns of a warp's 32 rows, a row a lane, between registers and global memory through the warp's staging rows,
-// so that global accesses run along rows. `rows` of them exist, and columns below `cols`.
+// Stores 32 columns of a warp's 32 rows, a row a lane, through the warp's staging rows, so that global accesses run
+// along rows. `rows` of them exist, and columns below `cols`.
 template <class Out>
 struct Rows32 {
   using Traits = OutTraits<Out>;
@@ -214,31 +219,96 @@ struct Rows32 {
     }
   }
 
-  __device__ static void load(uint8_t* staging, int lane, const Out* base, long long ld, int rows, int col0, int cols,
-                              bool wide, float* v) {
-    __syncwarp();
-    if (wide) {
-      const int unit = lane % kUnits;
-      const int col = col0 + unit * Traits::kPerUnit;
+};
+
+// The SwiGLU epilogues work on 64 bytes of a row of g and u at a time.
+template <class Out>
+constexpr int kSpan = 64 / static_cast<int>(sizeof(Out));
+
+// A warp's 32 rows of one span, in the order of whole rows (lane / 4 and a quarter of the row each).
+struct Span {
+  uint4 v[4];
+  template <class Out>
+  __device__ void load(int lane, const Out* base, long long ld, int rows, int col0, int cols) {
+    const int col = col0 + (lane % 4) * OutTraits<Out>::kPerUnit;
 #pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-        const int r = i * kRowsAtOnce + lane / kUnits;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < rows && col < cols) x = *reinterpret_cast<const uint4*>(base + r * ld + col);
-        *reinterpret_cast<uint4*>(staging + unit_at<kUnits>(r, unit)) = x;
-      }
-    } else {
-      const int unit = lane / Traits::kPerUnit, in = lane % Traits::kPerUnit;
-      for (int r = 0; r < 32; ++r)
-        reinterpret_cast<Out*>(staging + unit_at<kUnits>(r, unit))[in] =
-            r < rows && col0 + lane < cols ? base[r * ld + col0 + lane] : Traits::zero();
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + lane / 4;
+      v[i] = r < rows && col < cols ? *reinterpret_cast<const uint4*>(base + r * ld + col) : make_uint4(0, 0, 0, 0);
     }
-    __syncwarp();
+  }
+  __device__ void to_staging(uint8_t* staging, int lane) const {
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u)
-      Traits::unpack(*reinterpret_cast<const uint4*>(staging + unit_at<kUnits>(lane, u)), v + u * Traits::kPerUnit);
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(staging + unit_at<4>(i * 8 + lane / 4, lane % 4)) = v[i];
   }
 };
+
+template <class Out>
+__device__ __forceinline__ void row_from_staging(const uint8_t* staging, int lane, float (&v)[kSpan<Out>]) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    OutTraits<Out>::unpack(*reinterpret_cast<const uint4*>(staging + unit_at<4>(lane, u)), v + u * OutTraits<Out>::kPerUnit);
+}
+
+// Stores a span with padded rows.
+template <class Out>
+__device__ __forceinline__ void store_span(uint8_t* staging, int lane, Out* base, long long ld, int rows, int col0, int cols,
+                                           const float (&v)[kSpan<Out>]) {
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    *reinterpret_cast<uint4*>(staging + unit_at<4>(lane, u)) = OutTraits<Out>::pack(v + u * OutTraits<Out>::kPerUnit);
+  __syncwarp();
+  const int col = col0 + (lane % 4) * OutTraits<Out>::kPerUnit;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + lane / 4;
+    if (r < rows && col < cols)
+      *reinterpret_cast<uint4*>(base + r * ld + col) = *reinterpret_cast<const uint4*>(staging + unit_at<4>(r, lane % 4));
+  }
+}
+
+// Stores a span as an operand of the next product: with one plane the bf16 numbers themselves, else their parts (16
+// columns of fp32, 32 bytes a row and plane).
+template <int PLANES>
+__device__ __forceinline__ void store_operand(uint8_t* staging, int lane, __nv_bfloat16* base, long long plane, long long ld,
+                                              int rows, int col0, int cols,
+                                              const float (&v)[PLANES == 1 ? 32 : 16]) {
+  if constexpr (PLANES == 1) {
+    store_span<__nv_bfloat16>(staging, lane, base, ld, rows, col0, cols, v);
+  } else {
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      __nv_bfloat16 part[8][3];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) split(v[u * 8 + j], part[j]);
+#pragma unroll
+      for (int pl = 0; pl < PLANES; ++pl) {
+        uint4 x;
+        uint32_t* w = &x.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __nv_bfloat162 two = __halves2bfloat162(part[2 * j][pl], part[2 * j + 1][pl]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&two);
+        }
+        *reinterpret_cast<uint4*>(staging + pl * 1024 + unit_at<2>(lane, u)) = x;
+      }
+    }
+    __syncwarp();
+    const int col = col0 + (lane % 2) * 8;
+#pragma unroll
+    for (int pl = 0; pl < PLANES; ++pl) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = i * 16 + lane / 2;
+        if (r < rows && col < cols)
+          *reinterpret_cast<uint4*>(base + pl * plane + r * ld + col) =
+              *reinterpret_cast<const uint4*>(staging + pl * 1024 + unit_at<2>(r, lane % 2));
+      }
+    }
+  }
+}
 
 struct Tile {
   int expert;     // == experts: rows that nobody owns
@@ -364,6 +434,9 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
     return t;
   };
 
+  if (warp < kEpiWarp0) {
+    if constexpr (PLANES > 1) regs_decrease<Cfg::kRegsControl>();
+  }
   if (warp == 0) {
     // -------------------------------------------------------------- loads
     if (elect_one_sync()) {
@@ -526,17 +599,18 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
     }
   } else if (warp >= kEpiWarp0) {
     // -------------------------------------------------------------- epilogue
+    if constexpr (PLANES > 1) regs_increase<Cfg::kRegsEpilogue>();
     constexpr int kCols = Cfg::kBN / 2;  // columns of a thread: half a row of the tile
-    constexpr int kGroups = kCols / 32;
+    constexpr int kSpanCols = kSpan<Out>;
     const int quarter = warp % 4, half = (warp - kEpiWarp0) / 4;
     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     uint8_t* mine = staging + (warp - kEpiWarp0) * kStageOutBytes;
-    // Tensor-memory column of a thread's group: for SwiGLU its gate columns, then the same up columns.
-    auto tmem_col = [&](int g) {
+    // Tensor-memory column of a thread's column c: for SwiGLU first its gate columns, then the same up columns.
+    auto tmem_col = [&](int c) {
       if constexpr (EPI == kSwiGLU)
-        return (g < kGroups / 2 ? 0 : Cfg::kBN / 2) + half * (kCols / 2) + 32 * (g % (kGroups / 2));
+        return (c < kCols / 2 ? 0 : Cfg::kBN / 2) + half * (kCols / 2) + c % (kCols / 2);
       else
-        return half * kCols + 32 * g;
+        return half * kCols + c;
     };
     Position<2> at;
     bool ok = true;
@@ -545,6 +619,17 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       const Tile t = tile_at(unit, e);
       const int row0 = t.row0 + quarter * 32;
       const int rows = min(max(t.row_end - row0, 0), 32);
+      const long long first = (WEIGHTS ? static_cast<long long>(t.expert) * p.m : 0) + row0;
+      // g and u of the first span travel while the MMAs run.
+      Span next_g, next_u;
+      const Out* g_rows = static_cast<const Out*>(p.in[0]) + first * p.ld_in;
+      const Out* u_rows = static_cast<const Out*>(p.in[1]) + first * p.ld_in;
+      if constexpr (EPI == kSwiGLUBwd) {
+        if (t.steps > 0) {
+          next_g.load(lane, g_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
+          next_u.load(lane, u_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
+        }
+      }
       float acc[PLANES > 1 ? kCols : 1];
       int buf = 0;
       if constexpr (PLANES > 1) {
@@ -556,12 +641,12 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int g = 0; g < kGroups; ++g) {
+          for (int c = 0; c < kCols; c += 32) {
             uint32_t v[32];
-            tmem_ld32(taddr + buf * Cfg::kBN + tmem_col(g), v);
+            tmem_ld32(taddr + buf * Cfg::kBN + tmem_col(c), v);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[g * 32 + i] += __uint_as_float(v[i]);
+            for (int i = 0; i < 32; ++i) acc[c + i] += __uint_as_float(v[i]);
           }
           tc_fence_before();
           __syncwarp();
@@ -576,67 +661,80 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
         tc_fence_after();
       }
       if (!ok) break;
-      auto group = [&](int g, float (&v)[32]) {
+      // Columns [c, c + N) of the thread's row of the tile.
+      auto columns = [&](int c, auto& v) {
+        constexpr int N = sizeof(v) / sizeof(float);
         if constexpr (PLANES > 1) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = acc[g * 32 + i];
+          for (int i = 0; i < N; ++i) v[i] = acc[c + i];
         } else if (t.steps > 0) {
+          static_assert(N == 32, "one tensor-memory load");
           uint32_t raw[32];
-          tmem_ld32(taddr + buf * Cfg::kBN + tmem_col(g), raw);
+          tmem_ld32(taddr + buf * Cfg::kBN + tmem_col(c), raw);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+          for (int i = 0; i < N; ++i) v[i] = __uint_as_float(raw[i]);
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          for (int i = 0; i < N; ++i) v[i] = 0.f;
         }
       };
-      const long long ld = p.n;
-      const long long first = (WEIGHTS ? static_cast<long long>(t.expert) * p.m : 0) + row0;
-      auto out = [&](int o) { return static_cast<Out*>(p.out[o]) + first * ld; };
-      auto in = [&](int i) { return static_cast<const Out*>(p.in[i]) + first * ld; };
       if constexpr (EPI == kStore) {
+        Out* out = static_cast<Out*>(p.out[t.output]) + first * p.ld[0];
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
+        for (int c = 0; c < kCols; c += 32) {
           float v[32];
-          group(g, v);
-          Rows32<Out>::store(mine, lane, out(t.output), ld, rows, t.n0 + half * kCols + 32 * g, p.n, p.wide, v);
+          columns(c, v);
+          Rows32<Out>::store(mine, lane, out, p.ld[0], rows, t.n0 + half * kCols + c, p.n, p.wide, v);
         }
       } else if constexpr (EPI == kSwiGLU) {
 #pragma unroll
-        for (int g = 0; g < kGroups / 2; ++g) {
-          float gate[32], up[32];
-          group(g, gate);
-          group(g + kGroups / 2, up);
-          const int col = t.n0 + half * (kCols / 2) + 32 * g;
-          Rows32<Out>::store(mine, lane, out(0), ld, rows, col, p.n, p.wide, gate);
-          Rows32<Out>::store(mine, lane, out(1), ld, rows, col, p.n, p.wide, up);
+        for (int c = 0; c < kCols / 2; c += kSpanCols) {
+          float gate[kSpanCols], up[kSpanCols];
+          columns(c, gate);
+          columns(c + kCols / 2, up);
+          const int col = t.n0 + half * (kCols / 2) + c;
+          store_span<Out>(mine, lane, static_cast<Out*>(p.out[0]) + first * p.ld[0], p.ld[0], rows, col, p.n, gate);
+          store_span<Out>(mine, lane, static_cast<Out*>(p.out[1]) + first * p.ld[1], p.ld[1], rows, col, p.n, up);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) up[i] *= gate[i] / (1.f + __expf(-gate[i]));
-          Rows32<Out>::store(mine, lane, out(2), ld, rows, col, p.n, p.wide, up);
+          for (int i = 0; i < kSpanCols; ++i) up[i] *= gate[i] / (1.f + __expf(-gate[i]));
+          store_operand<PLANES>(mine, lane, static_cast<__nv_bfloat16*>(p.out[2]) + first * p.ld[2], p.plane, p.ld[2], rows,
+                                col, p.n, up);
         }
       } else {
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          float dh[32], gate[32], up[32];
-          group(g, dh);
-          const int col = t.n0 + half * kCols + 32 * g;
+        for (int c = 0; c < kCols; c += kSpanCols) {
+          float d_gate[kSpanCols], d_up[kSpanCols];
+          const int col = t.n0 + half * kCols + c;
           if (t.steps > 0) {
-            Rows32<Out>::load(mine, lane, in(0), ld, rows, col, p.n, p.wide, gate);
-            Rows32<Out>::load(mine, lane, in(1), ld, rows, col, p.n, p.wide, up);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float sig = 1.f / (1.f + __expf(-gate[i]));
-              const float d_up = dh[i] * gate[i] * sig;
-              dh[i] = dh[i] * up[i] * sig * (1.f + gate[i] * (1.f - sig));
-              up[i] = d_up;
+            __syncwarp();
+            next_g.to_staging(mine, lane);
+            next_u.to_staging(mine + 2048, lane);
+            if (c + kSpanCols < kCols) {
+              next_g.load(lane, g_rows, p.ld_in, rows, col + kSpanCols, p.n);
+              next_u.load(lane, u_rows, p.ld_in, rows, col + kSpanCols, p.n);
             }
+            __syncwarp();
+            columns(c, d_gate);  // dh
+            float g[kSpanCols];
+            row_from_staging<Out>(mine, lane, g);
+#pragma unroll
+            for (int i = 0; i < kSpanCols; ++i) {
+              const float sig = 1.f / (1.f + __expf(-g[i]));
+              d_up[i] = d_gate[i] * g[i] * sig;
+              d_gate[i] *= sig * (1.f + g[i] * (1.f - sig));
+            }
+            row_from_staging<Out>(mine + 2048, lane, g);  // u
+#pragma unroll
+            for (int i = 0; i < kSpanCols; ++i) d_gate[i] *= g[i];
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) up[i] = 0.f;
+            for (int i = 0; i < kSpanCols; ++i) d_gate[i] = d_up[i] = 0.f;
           }
-          Rows32<Out>::store(mine, lane, out(0), ld, rows, col, p.n, p.wide, dh);
-          Rows32<Out>::store(mine, lane, out(1), ld, rows, col, p.n, p.wide, up);
+          store_operand<PLANES>(mine, lane, static_cast<__nv_bfloat16*>(p.out[0]) + first * p.ld[0], p.plane, p.ld[0], rows,
+                                col, p.n, d_gate);
+          store_operand<PLANES>(mine, lane, static_cast<__nv_bfloat16*>(p.out[1]) + first * p.ld[1], p.plane, p.ld[1], rows,
+                                col, p.n, d_up);
         }
       }
       if (PLANES == 1 && t.steps > 0) {

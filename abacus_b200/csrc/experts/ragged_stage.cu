@@ -6,24 +6,11 @@
 #include <cuda_bf16.h>
 #include "../common/sm100.cuh"
 #include "ragged.h"
+#include "split.cuh"
 
 namespace abacus {
 namespace ragged {
 namespace {
-
-// x = h + m + l with each part the rounded remainder of those before. An
-// infinite or NaN x is h alone; a finite one too large to round up to bf16 is
-// cut instead, so that it stays finite.
-__device__ __forceinline__ void split(float x, int planes, __nv_bfloat16 (&part)[3]) {
-  const bool finite = isfinite(x);
-  float h = __bfloat162float(__float2bfloat16_rn(x));
-  if (finite && !isfinite(h)) h = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-  part[0] = __float2bfloat16_rn(h);
-  const float r = finite ? x - h : 0.f;
-  const float m = __bfloat162float(__float2bfloat16_rn(r));
-  part[1] = __float2bfloat16_rn(m);
-  part[2] = __float2bfloat16_rn(r - m);
-}
 
 __global__ void __launch_bounds__(256) stage_kernel(const StageParams p, bool vec, long long groups) {
   const long long per_row = p.ld / 8;
@@ -53,7 +40,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageParams p, bool ve
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         __nv_bfloat16 part[3];
-        split(x[j], p.planes, part);
+        split(x[j], part);
 #pragma unroll
         for (int q = 0; q < 3; ++q) out[q][j] = part[q];
       }

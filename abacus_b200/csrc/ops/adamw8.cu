@@ -40,6 +40,7 @@ namespace {
 
 constexpr int kBlock = 256;    // elements that share a scale (one warp)
 constexpr int kWarps = 8;      // blocks of a tensor taken by one CTA
+constexpr unsigned kInfinity = 0x7f800000u;
 constexpr int kTensors = 128;  // tensors of one launch (their table is the kernel's argument)
 
 struct Adam8Batch {
@@ -57,7 +58,7 @@ struct Adam8Batch {
 static_assert(sizeof(Adam8Batch) < 16 * 1024, "the table has to fit the kernel's arguments");
 
 struct Adam8Scalars {
-  float b1, c1, b2, c2, eps, decay, step_size, root_correction;
+  float b1, c1, b2, c2, eps, decay, step_size;
   unsigned step_mix;
 };
 
@@ -68,9 +69,18 @@ __device__ __forceinline__ unsigned mix(unsigned element, unsigned step_mix) {
   return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ unsigned magnitude(float x) {
-  const unsigned b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;  // infinities and NaN set no scale
+__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ unsigned finite_magnitude(float x) {
+  const unsigned b = magnitude(x);
+  return b < kInfinity ? b : 0u;  // infinities and NaN set no scale
+}
+
+// The special-function unit's root (within 2^-22): a last-bit error of u is far below its rounding to 8 bits, and
+// the correctly rounded root is a dozen instructions in a kernel that is short of issue slots.
+__device__ __forceinline__ float root(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // |x| on e4m3's grid, stochastically: 20 mantissa bits go, after 16 random bits
@@ -155,18 +165,33 @@ __global__ void __launch_bounds__(kWarps * 32) adamw8_kernel(const __grid_consta
       const float gi = g[h][e];
       const float mi = __fadd_rn(__fmul_rn(m[h][e] * ms, s.b1), __fmul_rn(gi, s.c1));
       const float uo = u[h][e] * us;
-      const float ui = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(uo, uo), s.b2), __fmul_rn(__fmul_rn(gi, gi), s.c2)));
-      const float ratio = __fdiv_rn(mi, __fdiv_rn(ui, s.root_correction) + s.eps);
-      w[h][e] = w[h][e] * s.decay - ratio * s.step_size;
+      const float ui = root(__fadd_rn(__fmul_rn(__fmul_rn(uo, uo), s.b2), __fmul_rn(__fmul_rn(gi, gi), s.c2)));
+      w[h][e] = w[h][e] * s.decay - __fdividef(mi * s.step_size, ui + s.eps);
       m[h][e] = mi;
       u[h][e] = ui;
       m_top = max(m_top, magnitude(mi));
       u_top = max(u_top, magnitude(ui));
     }
   }
+  m_top = __reduce_max_sync(0xffffffffu, m_top);
+  u_top = __reduce_max_sync(0xffffffffu, u_top);
+  const bool spoilt = max(m_top, u_top) >= kInfinity;  // somewhere in this block
+  if (spoilt) {
+    m_top = u_top = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m_top = max(m_top, finite_magnitude(m[h][e]));
+        u_top = max(u_top, finite_magnitude(u[h][e]));
+      }
+    }
+    m_top = __reduce_max_sync(0xffffffffu, m_top);
+    u_top = __reduce_max_sync(0xffffffffu, u_top);
+  }
   // Biased exponents of the scales; 1 (2^-126) is the smallest normal one.
-  const int me = max(static_cast<int>(__reduce_max_sync(0xffffffffu, m_top) >> 23) - 7, 1);
-  const int ue = max(static_cast<int>(__reduce_max_sync(0xffffffffu, u_top) >> 23) - 7, 1);
+  const int me = max(static_cast<int>(m_top >> 23) - 7, 1);
+  const int ue = max(static_cast<int>(u_top >> 23) - 7, 1);
   const float m_inv = __uint_as_float(static_cast<unsigned>(254 - me) << 23);
   const float u_inv = __uint_as_float(static_cast<unsigned>(254 - ue) << 23);
   if (lane == 0) {
@@ -181,11 +206,16 @@ __global__ void __launch_bounds__(kWarps * 32) adamw8_kernel(const __grid_consta
     for (int e = 0; e < 4; ++e) {
       const unsigned noise = mix(static_cast<unsigned>(begin + i + e), s.step_mix);
       const float ma = fabsf(m[h][e]) * m_inv, ua = u[h][e] * u_inv;
-      const float mg = copysignf(to_grid(ma, noise & 0xffffu), m[h][e]);
-      const float ug = to_grid(ua, noise >> 16);
+      mq[e] = copysignf(to_grid(ma, noise & 0xffffu), m[h][e]);
+      uq[e] = fmaxf(to_grid(ua, noise >> 16), ua > 0.f ? 0.001953125f : 0.f);
+    }
+    if (spoilt) {
       const float nan = __uint_as_float(0x7fffffffu);
-      mq[e] = isfinite(m[h][e]) ? mg : nan;
-      uq[e] = !isfinite(u[h][e]) ? nan : ua > 0.f ? fmaxf(ug, 0.001953125f) : ug;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (magnitude(m[h][e]) >= kInfinity) mq[e] = nan;
+        if (magnitude(u[h][e]) >= kInfinity) uq[e] = nan;
+      }
     }
     const uint32_t mc = pack4(mq), uc = pack4(uq);
     if (whole) {
@@ -225,10 +255,11 @@ void adamw8_step(const std::vector<torch::Tensor>& weights, const std::vector<to
   s.c1 = static_cast<float>(1.0 - beta1);
   s.b2 = static_cast<float>(beta2);
   s.c2 = static_cast<float>(1.0 - beta2);
-  s.eps = static_cast<float>(eps);
+  // a m / (u / c + eps) = (a c) m / (u + eps c): one division an element.
+  const double c = std::sqrt(1.0 - std::pow(beta2, static_cast<double>(step)));
+  s.eps = static_cast<float>(eps * c);
   s.decay = static_cast<float>(1.0 - lr * weight_decay);
-  s.step_size = static_cast<float>(lr / (1.0 - std::pow(beta1, static_cast<double>(step))));
-  s.root_correction = static_cast<float>(std::sqrt(1.0 - std::pow(beta2, static_cast<double>(step))));
+  s.step_size = static_cast<float>(lr * c / (1.0 - std::pow(beta1, static_cast<double>(step))));
   s.step_mix = static_cast<unsigned>(static_cast<uint64_t>(step) * 0x7F4A7C15ull);
   const auto stream = at::cuda::getCurrentCUDAStream();
   // Every tensor is looked at before the first is changed.

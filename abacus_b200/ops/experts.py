@@ -156,14 +156,14 @@ def _planes(t: torch.Tensor) -> int:
     return 1 if t.dtype == torch.bfloat16 else 3 if precision.passes() == 3 else 2
 
 
-def _operand(t: torch.Tensor) -> torch.Tensor:
+def _operand(t: torch.Tensor, planes: int | None = None) -> torch.Tensor:
     """``t`` as the product kernels read it: bf16 planes first, rows 16-byte aligned. bf16 tensors laid out so already
-    are used in place."""
+    are used in place. A backward pass gives the forward's number of planes, whatever the precision is by then."""
     if t.dtype == torch.bfloat16 and t.stride(-1) == 1 and t.data_ptr() % 16 == 0:
         aligned = all(t.shape[d] <= 1 or (t.stride(d) % 8 == 0 and t.stride(d) > 0) for d in range(t.ndim - 1))
         if aligned and (t.shape[-2] <= 1 or t.stride(-2) >= t.shape[-1]):
             return t.unsqueeze(0)
-    return ext().ragged_stage(t, _planes(t))
+    return ext().ragged_stage(t, planes or _planes(t))
 
 
 def _cpu_spans(offsets: torch.Tensor) -> list[tuple[int, int]]:
@@ -174,6 +174,7 @@ def _cpu_spans(offsets: torch.Tensor) -> list[tuple[int, int]]:
 class _RaggedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
+        ctx.planes = _planes(x)
         ctx.save_for_backward(x, w, offsets)
         y = torch.empty(x.shape[0], w.shape[2], dtype=x.dtype, device=x.device)
         ext().ragged_rows([_operand(x)], [_operand(w)], offsets, y, False)
@@ -183,44 +184,57 @@ class _RaggedMatmul(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
         dx = dw = None
-        dy = _operand(dy)
+        dy = _operand(dy, ctx.planes)
         if ctx.needs_input_grad[0]:
             dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            ext().ragged_rows([dy], [_operand(w)], offsets, dx, True)
+            ext().ragged_rows([dy], [_operand(w, ctx.planes)], offsets, dx, True)
         if ctx.needs_input_grad[1]:
             dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
-            ext().ragged_weights(_operand(x), [dy], offsets, [dw])
+            ext().ragged_weights(_operand(x, ctx.planes), [dy], offsets, [dw])
         return dx, dw, None
 
 
+def _padded(planes: int | None, rows: int, cols: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """Empty ([planes,] rows, cols) whose rows start at 16-byte boundaries."""
+    unit = 8 if dtype == torch.bfloat16 else 4
+    shape = (rows, -(-cols // unit) * unit)
+    t = torch.empty(shape if planes is None else (planes, *shape), dtype=dtype, device=device)
+    return t if shape[1] == cols else t[..., :cols]
+
+
 class _RaggedSwiGLU(torch.autograd.Function):
+    """The kernels write h and the gradients of gate and up as the operands (bf16 planes) of the products that read
+    them; the operands of x and h are kept for the backward in place of the tensors."""
+
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, offsets):
-        rows, hidden = x.shape[0], w_gate.shape[2]
-        g, u, h = (torch.empty(rows, hidden, dtype=x.dtype, device=x.device) for _ in range(3))
-        ext().ragged_swiglu(_operand(x), _operand(w_gate), _operand(w_up), offsets, g, u, h)
+        rows, hidden, planes = x.shape[0], w_gate.shape[2], _planes(x)
+        g, u = (_padded(None, rows, hidden, x.dtype, x.device) for _ in range(2))
+        h = _padded(planes, rows, hidden, torch.bfloat16, x.device)
         y = torch.empty(rows, w_down.shape[2], dtype=x.dtype, device=x.device)
-        ext().ragged_rows([_operand(h)], [_operand(w_down)], offsets, y, False)
+        x = _operand(x)
+        ext().ragged_swiglu(x, _operand(w_gate), _operand(w_up), offsets, g, u, h)
+        ext().ragged_rows([h], [_operand(w_down)], offsets, y, False)
         ctx.save_for_backward(x, w_gate, w_up, w_down, offsets, g, u, h)
         return y
 
     @staticmethod
     def backward(ctx, dy):
         x, w_gate, w_up, w_down, offsets, g, u, h = ctx.saved_tensors
-        dy = _operand(dy)
-        dg, du = torch.empty_like(g), torch.empty_like(u)
-        ext().ragged_swiglu_bwd(dy, _operand(w_down), offsets, g, u, dg, du)
+        planes, (rows, hidden) = h.shape[0], g.shape
+        dy = _operand(dy, planes)
+        dg, du = (_padded(planes, rows, hidden, torch.bfloat16, dy.device) for _ in range(2))
+        ext().ragged_swiglu_bwd(dy, _operand(w_down, planes), offsets, g, u, dg, du)
         grads = [None] * 5
-        dg, du = _operand(dg), _operand(du)
         if ctx.needs_input_grad[0]:
-            grads[0] = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            ext().ragged_rows([dg, du], [_operand(w_gate), _operand(w_up)], offsets, grads[0], True)
+            grads[0] = torch.empty(x.shape[1:], dtype=g.dtype, device=g.device)
+            ext().ragged_rows([dg, du], [_operand(w_gate, planes), _operand(w_up, planes)], offsets, grads[0], True)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             grads[1], grads[2] = (torch.empty(w.shape, dtype=w.dtype, device=w.device) for w in (w_gate, w_up))
-            ext().ragged_weights(_operand(x), [dg, du], offsets, [grads[1], grads[2]])
+            ext().ragged_weights(x, [dg, du], offsets, [grads[1], grads[2]])
         if ctx.needs_input_grad[3]:
             grads[3] = torch.empty(w_down.shape, dtype=w_down.dtype, device=w_down.device)
-            ext().ragged_weights(_operand(h), [dy], offsets, [grads[3]])
+            ext().ragged_weights(h, [dy], offsets, [grads[3]])
         return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad))
 
 
