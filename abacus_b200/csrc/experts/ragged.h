@@ -2,6 +2,7 @@
 // launchers shared by the kernel's translation units and the torch bindings.
 #pragma once
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 namespace abacus {
@@ -14,7 +15,7 @@ enum Epilogue : int { kStore = 0, kSwiGLU = 1, kSwiGLUBwd = 2 };
 // What a launch computes, over sorted rows r of expert e = [offsets[e], offsets[e + 1]):
 //  rows, store:      out0[r] = sum over segments s of a[s][r] B[s][e]
 //  rows, SwiGLU:     out0 = a B[0], out1 = a B[1], out2 = silu(out0) * out1
-//  rows, SwiGLU bwd: dh = a B[0]; out0 = dh u sig (1 + g (1 - sig)), out1 = dh g sig  (g = in0, u = in1)
+//  rows, SwiGLU bwd: dh = a B[0]; out0 = dh u sig (1 + g (1 - sig)), out1 = dh g sig  (g = in0, u = in1; one plane)
 //  weights:          out_o[e] = sum over r of a[r]^T b[o][r]
 // Rows at or after offsets[experts] get zeros. What the SwiGLU forms hand to the next product (its out2, its
 // backward's out0 and out1) is written as that product's operand, in bf16 planes; their rows and those of g and u are
@@ -68,6 +69,20 @@ struct StageParams {
   void* dst;
 };
 cudaError_t launch_stage(const StageParams& p, int sms, cudaStream_t stream);
+
+// The SwiGLU derivative of the fp32 forms, whose product writes dh: (rows, ld) fp32 dh, g and u to (planes, rows, ld_out)
+// bf16 parts of the gradients of gate and up. ld is a multiple of 4, ld_out the next multiple of 8 of cols.
+struct SwiGLUBwdParams {
+  const float* dh;
+  const float* g;
+  const float* u;
+  long long ld;
+  long long rows, cols, ld_out;
+  int planes;
+  __nv_bfloat16* dg;
+  __nv_bfloat16* du;
+};
+cudaError_t launch_swiglu_bwd(const SwiGLUBwdParams& p, int sms, cudaStream_t stream);
 
 }  // namespace ragged
 }  // namespace abacus

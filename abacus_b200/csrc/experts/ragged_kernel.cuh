@@ -225,30 +225,14 @@ struct Rows32 {
 template <class Out>
 constexpr int kSpan = 64 / static_cast<int>(sizeof(Out));
 
-// A warp's 32 rows of one span, in the order of whole rows (lane / 4 and a quarter of the row each).
+// A warp's 32 rows of one bf16 span, in the order of whole rows: lane / 4 and a quarter of the row each.
 struct Span {
   uint4 v[4];
-  template <class Out>
-  __device__ void load(int lane, const Out* base, long long ld, int rows, int col0, int cols) {
-    const int col = col0 + (lane % 4) * OutTraits<Out>::kPerUnit;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + lane / 4;
-      v[i] = r < rows && col < cols ? *reinterpret_cast<const uint4*>(base + r * ld + col) : make_uint4(0, 0, 0, 0);
-    }
-  }
-  __device__ void to_staging(uint8_t* staging, int lane) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(staging + unit_at<4>(i * 8 + lane / 4, lane % 4)) = v[i];
+  __device__ void load_quarter(int i, int lane, const __nv_bfloat16* base, long long ld, int rows, int col0, int cols) {
+    const int col = col0 + (lane % 4) * 8, r = i * 8 + lane / 4;
+    v[i] = r < rows && col < cols ? *reinterpret_cast<const uint4*>(base + r * ld + col) : make_uint4(0, 0, 0, 0);
   }
 };
-
-template <class Out>
-__device__ __forceinline__ void row_from_staging(const uint8_t* staging, int lane, float (&v)[kSpan<Out>]) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    OutTraits<Out>::unpack(*reinterpret_cast<const uint4*>(staging + unit_at<4>(lane, u)), v + u * OutTraits<Out>::kPerUnit);
-}
 
 // Stores a span with padded rows.
 template <class Out>
@@ -280,20 +264,10 @@ __device__ __forceinline__ void store_operand(uint8_t* staging, int lane, __nv_b
     __syncwarp();
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      __nv_bfloat16 part[8][3];
+      uint4 words[3];
+      split_eight(v + u * 8, words);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) split(v[u * 8 + j], part[j]);
-#pragma unroll
-      for (int pl = 0; pl < PLANES; ++pl) {
-        uint4 x;
-        uint32_t* w = &x.x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const __nv_bfloat162 two = __halves2bfloat162(part[2 * j][pl], part[2 * j + 1][pl]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&two);
-        }
-        *reinterpret_cast<uint4*>(staging + pl * 1024 + unit_at<2>(lane, u)) = x;
-      }
+      for (int pl = 0; pl < PLANES; ++pl) *reinterpret_cast<uint4*>(staging + pl * 1024 + unit_at<2>(lane, u)) = words[pl];
     }
     __syncwarp();
     const int col = col0 + (lane % 2) * 8;
@@ -309,6 +283,10 @@ __device__ __forceinline__ void store_operand(uint8_t* staging, int lane, __nv_b
     }
   }
 }
+
+// Within 2^-21: far inside the rounding of what it is multiplied into, and a quarter of the instructions of a correctly
+// rounded quotient.
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
 struct Tile {
   int expert;     // == experts: rows that nobody owns
@@ -620,14 +598,15 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       const int row0 = t.row0 + quarter * 32;
       const int rows = min(max(t.row_end - row0, 0), 32);
       const long long first = (WEIGHTS ? static_cast<long long>(t.expert) * p.m : 0) + row0;
-      // g and u of the first span travel while the MMAs run.
+      // g and u of the SwiGLU backward travel a span ahead, the first one's while the MMAs run.
       Span next_g, next_u;
-      const Out* g_rows = static_cast<const Out*>(p.in[0]) + first * p.ld_in;
-      const Out* u_rows = static_cast<const Out*>(p.in[1]) + first * p.ld_in;
+      const __nv_bfloat16* g_rows = static_cast<const __nv_bfloat16*>(p.in[0]) + first * p.ld_in;
+      const __nv_bfloat16* u_rows = static_cast<const __nv_bfloat16*>(p.in[1]) + first * p.ld_in;
       if constexpr (EPI == kSwiGLUBwd) {
-        if (t.steps > 0) {
-          next_g.load(lane, g_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
-          next_u.load(lane, u_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          next_g.load_quarter(i, lane, g_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
+          next_u.load_quarter(i, lane, u_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
         }
       }
       float acc[PLANES > 1 ? kCols : 1];
@@ -661,12 +640,16 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
         tc_fence_after();
       }
       if (!ok) break;
-      // Columns [c, c + N) of the thread's row of the tile.
+      // Columns [c, c + N) of the thread's row of the tile; the loops below go up by N. Their bodies stay loops (unrolled,
+      // they outgrow the instruction cache: the SwiGLU backward took 865 us where the loop took 654, 32768 rows of
+      // 2048 -> 5632), so with sums in registers the next N columns are moved to the front.
       auto columns = [&](int c, auto& v) {
         constexpr int N = sizeof(v) / sizeof(float);
         if constexpr (PLANES > 1) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = acc[c + i];
+          for (int i = 0; i < N; ++i) v[i] = acc[i];
+#pragma unroll
+          for (int i = 0; i + N < kCols; ++i) acc[i] = acc[i + N];
         } else if (t.steps > 0) {
           static_assert(N == 32, "one tensor-memory load");
           uint32_t raw[32];
@@ -681,60 +664,80 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       };
       if constexpr (EPI == kStore) {
         Out* out = static_cast<Out*>(p.out[t.output]) + first * p.ld[0];
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < kCols; c += 32) {
           float v[32];
           columns(c, v);
           Rows32<Out>::store(mine, lane, out, p.ld[0], rows, t.n0 + half * kCols + c, p.n, p.wide, v);
         }
       } else if constexpr (EPI == kSwiGLU) {
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < kCols / 2; c += kSpanCols) {
           float gate[kSpanCols], up[kSpanCols];
-          columns(c, gate);
-          columns(c + kCols / 2, up);
+          if constexpr (PLANES > 1) {
+            // Sums: gate and up columns side by side, a span of each at a time.
+#pragma unroll
+            for (int i = 0; i < kSpanCols; ++i) {
+              gate[i] = acc[i];
+              up[i] = acc[kCols / 2 + i];
+            }
+#pragma unroll
+            for (int i = 0; i + kSpanCols < kCols / 2; ++i) {
+              acc[i] = acc[i + kSpanCols];
+              acc[kCols / 2 + i] = acc[kCols / 2 + i + kSpanCols];
+            }
+          } else {
+            columns(c, gate);
+            columns(c + kCols / 2, up);
+          }
           const int col = t.n0 + half * (kCols / 2) + c;
           store_span<Out>(mine, lane, static_cast<Out*>(p.out[0]) + first * p.ld[0], p.ld[0], rows, col, p.n, gate);
           store_span<Out>(mine, lane, static_cast<Out*>(p.out[1]) + first * p.ld[1], p.ld[1], rows, col, p.n, up);
 #pragma unroll
-          for (int i = 0; i < kSpanCols; ++i) up[i] *= gate[i] / (1.f + __expf(-gate[i]));
+          for (int i = 0; i < kSpanCols; ++i) up[i] *= gate[i] * sigmoid(gate[i]);
           store_operand<PLANES>(mine, lane, static_cast<__nv_bfloat16*>(p.out[2]) + first * p.ld[2], p.plane, p.ld[2], rows,
                                 col, p.n, up);
         }
       } else {
+        // dh crosses the staging rows in fp32; g, u and both results stay in the order of whole rows. Each quarter of
+        // next_g and next_u is refilled for the next span as soon as it is used.
+        const long long ld = p.ld[0];
+        __nv_bfloat16* dg_rows = static_cast<__nv_bfloat16*>(p.out[0]) + first * ld;
+        __nv_bfloat16* du_rows = static_cast<__nv_bfloat16*>(p.out[1]) + first * ld;
+#pragma unroll 1
+        for (int c = 0; c < kCols; c += 32) {
+          float dh[32];
+          columns(c, dh);
+          __syncwarp();
 #pragma unroll
-        for (int c = 0; c < kCols; c += kSpanCols) {
-          float d_gate[kSpanCols], d_up[kSpanCols];
-          const int col = t.n0 + half * kCols + c;
-          if (t.steps > 0) {
-            __syncwarp();
-            next_g.to_staging(mine, lane);
-            next_u.to_staging(mine + 2048, lane);
-            if (c + kSpanCols < kCols) {
-              next_g.load(lane, g_rows, p.ld_in, rows, col + kSpanCols, p.n);
-              next_u.load(lane, u_rows, p.ld_in, rows, col + kSpanCols, p.n);
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<uint4*>(mine + unit_at<8>(lane, u)) = OutTraits<float>::pack(dh + 4 * u);
+          __syncwarp();
+          const int col = t.n0 + half * kCols + c + (lane % 4) * 8;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + lane / 4;
+            float d[8], g[8], u[8];
+            OutTraits<float>::unpack(*reinterpret_cast<const uint4*>(mine + unit_at<8>(r, (lane % 4) * 2)), d);
+            OutTraits<float>::unpack(*reinterpret_cast<const uint4*>(mine + unit_at<8>(r, (lane % 4) * 2 + 1)), d + 4);
+            OutTraits<__nv_bfloat16>::unpack(next_g.v[i], g);
+            OutTraits<__nv_bfloat16>::unpack(next_u.v[i], u);
+            if (c + 32 < kCols) {
+              next_g.load_quarter(i, lane, g_rows, p.ld_in, rows, t.n0 + half * kCols + c + 32, p.n);
+              next_u.load_quarter(i, lane, u_rows, p.ld_in, rows, t.n0 + half * kCols + c + 32, p.n);
             }
-            __syncwarp();
-            columns(c, d_gate);  // dh
-            float g[kSpanCols];
-            row_from_staging<Out>(mine, lane, g);
 #pragma unroll
-            for (int i = 0; i < kSpanCols; ++i) {
-              const float sig = 1.f / (1.f + __expf(-g[i]));
-              d_up[i] = d_gate[i] * g[i] * sig;
-              d_gate[i] *= sig * (1.f + g[i] * (1.f - sig));
+            for (int j = 0; j < 8; ++j) {
+              const float sig = sigmoid(g[j]);
+              const float through = d[j] * sig;
+              d[j] = through * u[j] * (1.f + g[j] * (1.f - sig));
+              g[j] *= through;
             }
-            row_from_staging<Out>(mine + 2048, lane, g);  // u
-#pragma unroll
-            for (int i = 0; i < kSpanCols; ++i) d_gate[i] *= g[i];
-          } else {
-#pragma unroll
-            for (int i = 0; i < kSpanCols; ++i) d_gate[i] = d_up[i] = 0.f;
+            if (r < rows && col < p.n) {
+              *reinterpret_cast<uint4*>(dg_rows + r * ld + col) = OutTraits<__nv_bfloat16>::pack(d);
+              *reinterpret_cast<uint4*>(du_rows + r * ld + col) = OutTraits<__nv_bfloat16>::pack(g);
+            }
           }
-          store_operand<PLANES>(mine, lane, static_cast<__nv_bfloat16*>(p.out[0]) + first * p.ld[0], p.plane, p.ld[0], rows,
-                                col, p.n, d_gate);
-          store_operand<PLANES>(mine, lane, static_cast<__nv_bfloat16*>(p.out[1]) + first * p.ld[1], p.plane, p.ld[1], rows,
-                                col, p.n, d_up);
         }
       }
       if (PLANES == 1 && t.steps > 0) {
@@ -795,7 +798,9 @@ cudaError_t launch_shape(const Params& p, const Shape& s, long long units, int s
                   : launch_one<PLANES, PAIR, false, false, kStore>(p, units, sms, stream);
   }
   if (s.epilogue == kSwiGLU && s.b_mn) return launch_one<PLANES, PAIR, false, true, kSwiGLU>(p, units, sms, stream);
-  if (s.epilogue == kSwiGLUBwd && !s.b_mn) return launch_one<PLANES, PAIR, false, false, kSwiGLUBwd>(p, units, sms, stream);
+  if constexpr (PLANES == 1) {
+    if (s.epilogue == kSwiGLUBwd && !s.b_mn) return launch_one<PLANES, PAIR, false, false, kSwiGLUBwd>(p, units, sms, stream);
+  }
   return cudaErrorInvalidValue;
 }
 
