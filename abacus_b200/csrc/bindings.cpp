@@ -41,16 +41,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cross_entropy_grad", &abacus::ops::cross_entropy_grad);
   m.def("adamw_step", &abacus::ops::adamw_step);
   m.def("adamw8_step", &abacus::ops::adamw8_step, "AdamW over many tensors with 8-bit moments");
-  m.def("expert_plan", &abacus::ops::expert_plan, "stable sort of routed assignments by expert");
-  m.def("expert_plan_parts", &abacus::ops::expert_plan_parts, "rows of expert_plan's workspace");
-  m.def("expert_dispatch", &abacus::ops::expert_dispatch, "token rows into expert order");
-  m.def("expert_combine", &abacus::ops::expert_combine, "(weighted) sum of each token's expert rows");
-  m.def("expert_combine_bwd", &abacus::ops::expert_combine_bwd, "gradients of the weighted sum");
+  m.def("expert_plan", &abacus::experts::plan, "stable sort of routed assignments by expert: offsets, order, slot");
+  m.def("expert_dispatch", &abacus::experts::dispatch, "token rows into expert order (differentiable)");
+  m.def("expert_combine", &abacus::experts::combine, "weighted sum of each token's expert rows (differentiable)");
+  m.def("ragged_matmul", &abacus::experts::matmul, "sorted rows times their experts' matrices (differentiable)");
+  m.def("ragged_swiglu_mlp", &abacus::experts::swiglu_mlp, "SwiGLU experts over sorted rows (differentiable)");
   m.def("ragged_stage", &abacus::ragged::stage, "bf16 planes of an operand of the ragged products");
-  m.def("ragged_rows", &abacus::ragged::rows, "sorted rows times their experts' matrices");
-  m.def("ragged_swiglu", &abacus::ragged::swiglu, "gate and up products with the SwiGLU epilogue");
+  m.def("ragged_rows", &abacus::ragged::rows, "sorted rows times their experts' matrices, staged operands");
+  m.def("ragged_swiglu", &abacus::ragged::swiglu, "gate and up products with the SwiGLU epilogue, staged operands");
   m.def("ragged_swiglu_bwd", &abacus::ragged::swiglu_bwd, "gradient through the down product with the SwiGLU derivative");
-  m.def("ragged_weights", &abacus::ragged::weights, "per-expert weight gradients over sorted rows");
+  m.def("ragged_weights", &abacus::ragged::weights, "per-expert weight gradients over sorted rows, staged operands");
   m.def("causal_softmax_fwd", &abacus::attn::causal_softmax_fwd, "in-place causal row softmax (materialised attention)");
   m.def("causal_softmax_bwd", &abacus::attn::causal_softmax_bwd, "in-place dS from P and dP (materialised attention)");
   m.def("flash_attn_fwd_cp", &abacus::attn::flash_attn_fwd_cp, "flash forward over peer-pushed K/V (context parallel)");

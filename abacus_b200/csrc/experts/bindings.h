@@ -1,6 +1,7 @@
-// Torch entry points of the ragged expert products (see ragged_bindings.cpp).
+// Torch entry points of the expert operators: the products (see ragged_bindings.cpp) ...
 #pragma once
 #include <torch/extension.h>
+#include <tuple>
 #include <vector>
 
 namespace abacus {
@@ -14,4 +15,14 @@ void swiglu_bwd(torch::Tensor dy, torch::Tensor w_down, torch::Tensor offsets, t
                 torch::Tensor dg, torch::Tensor du);
 void weights(torch::Tensor x, std::vector<torch::Tensor> dy, torch::Tensor offsets, std::vector<torch::Tensor> dw);
 }  // namespace ragged
+
+// Differentiable operators (see functions.cpp).
+namespace experts {
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> plan(torch::Tensor indices, int64_t n_experts);
+torch::Tensor dispatch(torch::Tensor x, torch::Tensor offsets, torch::Tensor slot);
+torch::Tensor combine(torch::Tensor ys, torch::Tensor weights, torch::Tensor offsets, torch::Tensor slot);
+torch::Tensor matmul(torch::Tensor x, torch::Tensor w, torch::Tensor offsets, int64_t fp32_planes);
+torch::Tensor swiglu_mlp(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, torch::Tensor w_down,
+                         torch::Tensor offsets, int64_t fp32_planes);
+}  // namespace experts
 }  // namespace abacus

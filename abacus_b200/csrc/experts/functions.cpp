@@ -1,0 +1,233 @@
+// The differentiable expert operators that abacus_b200/ops/experts.py exports for CUDA tensors: argument checks, workspaces
+// and autograd nodes around the kernels. They are C++ nodes because a short batch is bound by the host: the same nodes in
+// Python took 142 us for the routing of 256 tokens with its gradients, whose kernels take 17.
+//
+// None of them is differentiable twice; a backward pass that records a graph is refused.
+#include <torch/extension.h>
+#include <ATen/core/grad_mode.h>
+#include "../ops/expert_rows.h"
+#include "bindings.h"
+
+namespace abacus {
+namespace experts {
+namespace {
+
+using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool row_type(const Tensor& t) { return t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16; }
+
+void check_rows(const Tensor& t, const char* name, int64_t rows = -1) {
+  TORCH_CHECK_VALUE(t.dim() == 2 && row_type(t), name, " must be a 2-D fp32 or bf16 tensor, got ", t.sizes(), " ",
+                    t.scalar_type());
+  TORCH_CHECK_VALUE(rows < 0 || t.size(0) == rows, name, " must have ", rows, " rows, got ", t.size(0));
+}
+
+// Rows that a kernel can walk: unit inner stride, no overlap.
+Tensor walkable(const Tensor& t) {
+  return t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) ? t : t.contiguous();
+}
+
+void once_only(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, " is not differentiable twice (create_graph=True)");
+}
+
+void check_plan(const Tensor& offsets, const Tensor& slot, const Tensor& like) {
+  TORCH_CHECK_VALUE(offsets.device() == like.device() && slot.device() == like.device(),
+                    "the rows and the plan must be on one device");
+}
+
+// Sum over each token's kept choices, weighted or not.
+Tensor combine_rows(const Tensor& ys, c10::optional<Tensor> weights, const Tensor& slot) {
+  auto out = torch::empty({slot.size(0), ys.size(1)}, ys.options());
+  ops::expert_combine(ys, weights, slot, out);
+  return out;
+}
+
+struct Dispatch : torch::autograd::Function<Dispatch> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& offsets, const Tensor& slot) {
+    ctx->save_for_backward({slot});
+    auto xs = torch::empty({slot.numel(), x.size(1)}, x.options());
+    ops::expert_dispatch(walkable(x), slot, offsets, xs);
+    return xs;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("dispatch_tokens");
+    return {combine_rows(grads[0].contiguous(), c10::nullopt, ctx->get_saved_variables()[0]), Tensor(), Tensor()};
+  }
+};
+
+struct Combine : torch::autograd::Function<Combine> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& ys, const Tensor& weights, const Tensor& offsets,
+                        const Tensor& slot) {
+    ctx->save_for_backward({ys, weights, offsets, slot});
+    return combine_rows(ys, weights, slot);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("combine_tokens");
+    const auto saved = ctx->get_saved_variables();
+    auto dys = torch::empty_like(saved[0]), dweights = torch::empty_like(saved[1]);
+    ops::expert_combine_bwd(grads[0].contiguous(), saved[0], saved[1], saved[3], saved[2], dys, dweights);
+    return {dys, dweights, Tensor(), Tensor()};
+  }
+};
+
+// `t` as the product kernels read it: bf16 planes first, rows 16-byte aligned. bf16 tensors laid out so already are used in
+// place.
+Tensor operand(const Tensor& t, int64_t planes) {
+  const int64_t d = t.dim();
+  if (t.scalar_type() == torch::kBFloat16 && t.stride(d - 1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) {
+    bool aligned = t.size(d - 2) <= 1 || t.stride(d - 2) >= t.size(d - 1);
+    for (int64_t i = 0; i < d - 1; ++i) aligned = aligned && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) > 0));
+    if (aligned) return t.unsqueeze(0);
+  }
+  return ragged::stage(t, planes);
+}
+
+Tensor like_matrix(const Tensor& w) { return torch::empty(w.sizes(), w.options()); }
+
+// Empty ([planes,] rows, cols) whose rows start at 16-byte boundaries.
+Tensor padded(int64_t planes, int64_t rows, int64_t cols, torch::TensorOptions options) {
+  const int64_t unit = options.dtype() == torch::kBFloat16 ? 8 : 4, ld = (cols + unit - 1) / unit * unit;
+  const auto t = planes ? torch::empty({planes, rows, ld}, options) : torch::empty({rows, ld}, options);
+  return ld == cols ? t : t.narrow(-1, 0, cols);
+}
+
+struct RaggedMatmul : torch::autograd::Function<RaggedMatmul> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t planes) {
+    ctx->save_for_backward({x, w, offsets});
+    ctx->saved_data["planes"] = planes;
+    auto y = torch::empty({x.size(0), w.size(2)}, x.options());
+    ragged::rows({operand(x, planes)}, {operand(w, planes)}, offsets, y, false);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("ragged_matmul");
+    const auto saved = ctx->get_saved_variables();
+    const auto &x = saved[0], &w = saved[1], &offsets = saved[2];
+    const int64_t planes = ctx->saved_data["planes"].toInt();
+    const auto dy = operand(grads[0], planes);
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) {
+      dx = torch::empty(x.sizes(), x.options());
+      ragged::rows({dy}, {operand(w, planes)}, offsets, dx, true);
+    }
+    if (ctx->needs_input_grad(1)) {
+      dw = like_matrix(w);
+      ragged::weights(operand(x, planes), {dy}, offsets, {dw});
+    }
+    return {dx, dw, Tensor(), Tensor()};
+  }
+};
+
+// The kernels write h and the gradients of gate and up as the operands (bf16 planes) of the products that read them; the
+// operands of x and h are kept for the backward in place of the tensors.
+struct RaggedSwiGLU : torch::autograd::Function<RaggedSwiGLU> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
+                        const Tensor& w_down, const Tensor& offsets, int64_t planes) {
+    const int64_t rows = x.size(0), hidden = w_gate.size(2);
+    const auto g = padded(0, rows, hidden, x.options()), u = padded(0, rows, hidden, x.options());
+    const auto h = padded(planes, rows, hidden, x.options().dtype(torch::kBFloat16));
+    auto y = torch::empty({rows, w_down.size(2)}, x.options());
+    const auto xo = operand(x, planes);
+    ragged::swiglu(xo, operand(w_gate, planes), operand(w_up, planes), offsets, g, u, h);
+    ragged::rows({h}, {operand(w_down, planes)}, offsets, y, false);
+    ctx->save_for_backward({xo, w_gate, w_up, w_down, offsets, g, u, h});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once_only("ragged_swiglu_mlp");
+    const auto saved = ctx->get_saved_variables();
+    const auto &x = saved[0], &w_gate = saved[1], &w_up = saved[2], &w_down = saved[3], &offsets = saved[4], &g = saved[5],
+               &u = saved[6], &h = saved[7];
+    const int64_t planes = h.size(0), rows = g.size(0), hidden = g.size(1);
+    const auto dy = operand(grads[0], planes);
+    const auto dg = padded(planes, rows, hidden, h.options()), du = padded(planes, rows, hidden, h.options());
+    ragged::swiglu_bwd(dy, operand(w_down, planes), offsets, g, u, dg, du);
+    variable_list out(6);
+    if (ctx->needs_input_grad(0)) {
+      out[0] = torch::empty({rows, x.size(2)}, g.options());
+      ragged::rows({dg, du}, {operand(w_gate, planes), operand(w_up, planes)}, offsets, out[0], true);
+    }
+    if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+      Tensor dw_gate = like_matrix(w_gate), dw_up = like_matrix(w_up);
+      ragged::weights(x, {dg, du}, offsets, {dw_gate, dw_up});
+      if (ctx->needs_input_grad(1)) out[1] = dw_gate;
+      if (ctx->needs_input_grad(2)) out[2] = dw_up;
+    }
+    if (ctx->needs_input_grad(3)) {
+      out[3] = like_matrix(w_down);
+      ragged::weights(h, {dy}, offsets, {out[3]});
+    }
+    return out;
+  }
+};
+
+int64_t planes_of(const Tensor& x, int64_t fp32_planes) { return x.scalar_type() == torch::kBFloat16 ? 1 : fp32_planes; }
+
+void check_products(const Tensor& x, const Tensor& w, const char* name, int64_t in, int64_t out, const Tensor& offsets) {
+  const int64_t experts = offsets.numel() - 1;
+  TORCH_CHECK_VALUE(w.dim() == 3, name, " must be (experts, in, out), got ", w.sizes());
+  TORCH_CHECK_VALUE(w.scalar_type() == x.scalar_type() && w.size(0) == experts && w.size(1) == in && w.size(2) == out, name,
+                    " must be ", x.scalar_type(), " of shape [", experts, ", ", in, ", ", out, "], got ", w.scalar_type(),
+                    " ", w.sizes());
+  TORCH_CHECK_VALUE(w.device() == x.device() && offsets.device() == x.device(),
+                    "the rows, the matrices and the offsets must be on one device");
+  TORCH_CHECK_VALUE(in > 0 && out > 0, name, " has an empty dimension: ", w.sizes());
+}
+
+void check_offsets(const Tensor& offsets) {
+  TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 2 && offsets.scalar_type() == torch::kInt32,
+                    "offsets must be int32 of shape (experts + 1,), got ", offsets.sizes(), " ", offsets.scalar_type());
+}
+
+}  // namespace
+
+std::tuple<Tensor, Tensor, Tensor> plan(Tensor indices, int64_t n_experts) {
+  TORCH_CHECK_VALUE(indices.dim() == 2 && (indices.scalar_type() == torch::kInt64 || indices.scalar_type() == torch::kInt32),
+                    "indices must be a (tokens, choices) integer tensor, got ", indices.sizes(), " ", indices.scalar_type());
+  TORCH_CHECK_VALUE(n_experts >= 1, "n_experts must be at least 1, got ", n_experts);
+  const auto flat = indices.to(torch::kInt64).contiguous();
+  const int64_t n = flat.numel(), bins = n_experts + 1, parts = ops::expert_plan_parts(n);
+  // One allocation: offsets, order, slot, and the counts of the parts.
+  const auto ints = torch::empty({bins + 2 * n + (parts > 1 ? parts * bins : 0)}, flat.options().dtype(torch::kInt32));
+  const auto offsets = ints.narrow(0, 0, bins), order = ints.narrow(0, bins, n), slot = ints.narrow(0, bins + n, n);
+  ops::expert_plan(flat, n_experts, offsets, order, slot, ints.narrow(0, bins + 2 * n, ints.numel() - bins - 2 * n));
+  return {offsets, order, slot.view(indices.sizes())};
+}
+
+Tensor dispatch(Tensor x, Tensor offsets, Tensor slot) {
+  check_rows(x, "x", slot.size(0));
+  check_plan(offsets, slot, x);
+  return Dispatch::apply(x, offsets, slot);
+}
+
+Tensor combine(Tensor ys, Tensor weights, Tensor offsets, Tensor slot) {
+  check_rows(ys, "ys", slot.numel());
+  TORCH_CHECK_VALUE(weights.sizes() == slot.sizes() && weights.scalar_type() == torch::kFloat32,
+                    "weights must be fp32 of shape ", slot.sizes(), ", got ", weights.sizes(), " ", weights.scalar_type());
+  check_plan(offsets, slot, ys);
+  TORCH_CHECK_VALUE(weights.device() == ys.device(), "the rows and the weights must be on one device");
+  return Combine::apply(ys.contiguous(), weights.contiguous(), offsets, slot);
+}
+
+Tensor matmul(Tensor x, Tensor w, Tensor offsets, int64_t fp32_planes) {
+  check_rows(x, "x");
+  check_offsets(offsets);
+  check_products(x, w, "w", x.size(1), w.dim() == 3 ? w.size(2) : 0, offsets);
+  return RaggedMatmul::apply(x, w, offsets.contiguous(), planes_of(x, fp32_planes));
+}
+
+Tensor swiglu_mlp(Tensor x, Tensor w_gate, Tensor w_up, Tensor w_down, Tensor offsets, int64_t fp32_planes) {
+  check_rows(x, "x");
+  check_offsets(offsets);
+  const int64_t hidden = w_gate.dim() == 3 ? w_gate.size(2) : 0;
+  check_products(x, w_gate, "w_gate", x.size(1), hidden, offsets);
+  check_products(x, w_up, "w_up", x.size(1), hidden, offsets);
+  check_products(x, w_down, "w_down", hidden, w_down.dim() == 3 ? w_down.size(2) : 0, offsets);
+  return RaggedSwiGLU::apply(x, w_gate, w_up, w_down, offsets.contiguous(), planes_of(x, fp32_planes));
+}
+
+}  // namespace experts
+}  // namespace abacus
