@@ -39,7 +39,8 @@ namespace ops {
 namespace {
 
 constexpr int kBlock = 256;    // elements that share a scale (one warp)
-constexpr int kWarps = 8;      // blocks of a tensor taken by one CTA
+constexpr int kWarps = 8;      // of a CTA
+constexpr int kRounds = 4;     // blocks of a tensor taken by a warp of a large launch, to share finding the tensor
 constexpr unsigned kInfinity = 0x7f800000u;
 constexpr int kTensors = 128;  // tensors of one launch (their table is the kernel's argument)
 
@@ -54,6 +55,7 @@ struct Adam8Batch {
   unsigned first[kTensors + 1];  // first CTA of each tensor
   uint8_t g_bf16[kTensors], wide[kTensors];
   int count;
+  int rounds;  // blocks a warp
 };
 static_assert(sizeof(Adam8Batch) < 16 * 1024, "the table has to fit the kernel's arguments");
 
@@ -69,11 +71,14 @@ __device__ __forceinline__ unsigned mix(unsigned element, unsigned step_mix) {
   return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-__device__ __forceinline__ unsigned finite_magnitude(float x) {
-  const unsigned b = magnitude(x);
-  return b < kInfinity ? b : 0u;  // infinities and NaN set no scale
+// The larger of `top` and |x|, NaN if either is.
+__device__ __forceinline__ float largest(float top, float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(top), "f"(fabsf(x)));
+  return y;
 }
+// Over the warp, as bits (of numbers that are not negative, which order as their bits do, NaN last).
+__device__ __forceinline__ unsigned warp_top(float top) { return __reduce_max_sync(0xffffffffu, __float_as_uint(top)); }
 
 // The special-function unit's root (within 2^-22): a last-bit error of u is far below its rounding to 8 bits, and
 // the correctly rounded root is a dozen instructions in a kernel that is short of issue slots.
@@ -83,13 +88,23 @@ __device__ __forceinline__ float root(float x) {
   return y;
 }
 
-// |x| on e4m3's grid, stochastically: 20 mantissa bits go, after 16 random bits
-// were added at their top. Below 2^-6 the grid is 2^-9 throughout, which
-// adding 2^-6 first gives.
-__device__ __forceinline__ float to_grid(float a, unsigned noise16) {
-  const float base = a < 0.015625f ? 0.015625f : 0.f;
-  const unsigned bits = (__float_as_uint(a + base) + (noise16 << 4)) & 0xfff00000u;
-  return __uint_as_float(bits) - base;
+// The e4m3 code of x, rounded stochastically by 16 random bits; |x| < 256. Times 2^-120, e4m3's smallest normal number
+// (2^-6) is fp32's (2^-126) and the two formats' exponent fields agree, subnormal numbers included: the code is the upper
+// bits of the float, and adding the random bits below them before they are cut rounds up with the right probability and
+// carries into the exponent where it should. (fp32 keeps 20 bits below the grid; what it drops in a subnormal product is
+// rounded to nearest first.)
+__device__ __forceinline__ uint32_t to_code(float x, unsigned noise16) {
+  const uint32_t t = __float_as_uint(x * 0x1p-120f) + (noise16 << 4);
+  return (t << 4) | (t & 0x80000000u);  // in the top byte
+}
+__device__ __forceinline__ uint32_t to_code_positive(float x, unsigned noise16) {
+  return (__float_as_uint(x * 0x1p-120f) + (noise16 << 4)) >> 20;  // in the lowest byte
+}
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t (&x)[4]) {
+  return __byte_perm(__byte_perm(x[0], x[1], 0x0073), __byte_perm(x[2], x[3], 0x0073), 0x5410);
+}
+__device__ __forceinline__ uint32_t low_bytes(const uint32_t (&x)[4]) {
+  return __byte_perm(__byte_perm(x[0], x[1], 0x0040), __byte_perm(x[2], x[3], 0x0040), 0x5410);
 }
 
 __device__ __forceinline__ void unpack4(uint32_t codes, float (&x)[4]) {
@@ -99,13 +114,7 @@ __device__ __forceinline__ void unpack4(uint32_t codes, float (&x)[4]) {
   x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
 
-__device__ __forceinline__ uint32_t pack4(const float (&q)[4]) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
-
-__global__ void __launch_bounds__(kWarps * 32) adamw8_kernel(const __grid_constant__ Adam8Batch t, const Adam8Scalars s) {
+__global__ void __launch_bounds__(kWarps * 32, 5) adamw8_kernel(const __grid_constant__ Adam8Batch t, const Adam8Scalars s) {
   int lo = 0, hi = t.count - 1;  // the tensor of this CTA: the last whose first CTA is not after it
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
@@ -113,122 +122,131 @@ __global__ void __launch_bounds__(kWarps * 32) adamw8_kernel(const __grid_consta
     else hi = mid - 1;
   }
   const int lane = threadIdx.x % 32;
-  const long long block = static_cast<long long>(blockIdx.x - t.first[lo]) * kWarps + threadIdx.x / 32;
-  const long long begin = block * kBlock;
   const long long n = t.numel[lo];
-  if (begin >= n) return;
-  const bool whole = t.wide[lo] && begin + kBlock <= n;
-  float* wp = t.w[lo] + begin;
-  uint8_t* mp = t.m[lo] + begin;
-  uint8_t* up = t.u[lo] + begin;
+  long long block = static_cast<long long>(blockIdx.x - t.first[lo]) * (kWarps * t.rounds) + threadIdx.x / 32;
+#pragma unroll 1
+  for (int round = 0; round < t.rounds; ++round, block += kWarps) {
+    const long long begin = block * kBlock;
+    if (begin >= n) return;
+    const bool whole = t.wide[lo] && begin + kBlock <= n;
+    float* wp = t.w[lo] + begin;
+    uint8_t* mp = t.m[lo] + begin;
+    uint8_t* up = t.u[lo] + begin;
 
-  float w[2][4], g[2][4], m[2][4], u[2][4];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = h * 128 + lane * 4;
-    if (whole) {
-      const float4 w4 = *reinterpret_cast<const float4*>(wp + i);
-      w[h][0] = w4.x; w[h][1] = w4.y; w[h][2] = w4.z; w[h][3] = w4.w;
-      if (t.g_bf16[lo]) {
-        const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(t.g[lo]) + begin + i);
-        g[h][0] = __uint_as_float(raw.x << 16); g[h][1] = __uint_as_float(raw.x & 0xffff0000u);
-        g[h][2] = __uint_as_float(raw.y << 16); g[h][3] = __uint_as_float(raw.y & 0xffff0000u);
-      } else {
-        const float4 g4 = *reinterpret_cast<const float4*>(static_cast<const float*>(t.g[lo]) + begin + i);
-        g[h][0] = g4.x; g[h][1] = g4.y; g[h][2] = g4.z; g[h][3] = g4.w;
-      }
-      unpack4(*reinterpret_cast<const uint32_t*>(mp + i), m[h]);
-      unpack4(*reinterpret_cast<const uint32_t*>(up + i), u[h]);
-    } else {
-      uint32_t mc = 0, uc = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool in = begin + i + e < n;
-        w[h][e] = in ? wp[i + e] : 0.f;
-        g[h][e] = !in ? 0.f
-                  : t.g_bf16[lo] ? __bfloat162float(static_cast<const __nv_bfloat16*>(t.g[lo])[begin + i + e])
-                                 : static_cast<const float*>(t.g[lo])[begin + i + e];
-        mc |= in ? static_cast<uint32_t>(mp[i + e]) << (8 * e) : 0u;
-        uc |= in ? static_cast<uint32_t>(up[i + e]) << (8 * e) : 0u;
-      }
-      unpack4(mc, m[h]);
-      unpack4(uc, u[h]);
-    }
-  }
-
-  const float ms = t.m_scale[lo][block], us = t.u_scale[lo][block];
-  unsigned m_top = 0, u_top = 0;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float gi = g[h][e];
-      const float mi = __fadd_rn(__fmul_rn(m[h][e] * ms, s.b1), __fmul_rn(gi, s.c1));
-      const float uo = u[h][e] * us;
-      const float ui = root(__fadd_rn(__fmul_rn(__fmul_rn(uo, uo), s.b2), __fmul_rn(__fmul_rn(gi, gi), s.c2)));
-      w[h][e] = w[h][e] * s.decay - __fdividef(mi * s.step_size, ui + s.eps);
-      m[h][e] = mi;
-      u[h][e] = ui;
-      m_top = max(m_top, magnitude(mi));
-      u_top = max(u_top, magnitude(ui));
-    }
-  }
-  m_top = __reduce_max_sync(0xffffffffu, m_top);
-  u_top = __reduce_max_sync(0xffffffffu, u_top);
-  const bool spoilt = max(m_top, u_top) >= kInfinity;  // somewhere in this block
-  if (spoilt) {
-    m_top = u_top = 0;
+    // All loads first; the moments stay packed until they are used, and a weight leaves as soon as it is done.
+    float w[2][4], g[2][4], m[2][4], u[2][4];
+    uint32_t mc[2], uc[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      const int i = h * 128 + lane * 4;
+      if (whole) {
+        const float4 w4 = *reinterpret_cast<const float4*>(wp + i);
+        w[h][0] = w4.x; w[h][1] = w4.y; w[h][2] = w4.z; w[h][3] = w4.w;
+        if (t.g_bf16[lo]) {
+          const uint2 raw = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(t.g[lo]) + begin + i);
+          g[h][0] = __uint_as_float(raw.x << 16); g[h][1] = __uint_as_float(raw.x & 0xffff0000u);
+          g[h][2] = __uint_as_float(raw.y << 16); g[h][3] = __uint_as_float(raw.y & 0xffff0000u);
+        } else {
+          const float4 g4 = *reinterpret_cast<const float4*>(static_cast<const float*>(t.g[lo]) + begin + i);
+          g[h][0] = g4.x; g[h][1] = g4.y; g[h][2] = g4.z; g[h][3] = g4.w;
+        }
+        mc[h] = *reinterpret_cast<const uint32_t*>(mp + i);
+        uc[h] = *reinterpret_cast<const uint32_t*>(up + i);
+      } else {
+        mc[h] = uc[h] = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        m_top = max(m_top, finite_magnitude(m[h][e]));
-        u_top = max(u_top, finite_magnitude(u[h][e]));
+        for (int e = 0; e < 4; ++e) {
+          const bool in = begin + i + e < n;
+          w[h][e] = in ? wp[i + e] : 0.f;
+          g[h][e] = !in ? 0.f
+                    : t.g_bf16[lo] ? __bfloat162float(static_cast<const __nv_bfloat16*>(t.g[lo])[begin + i + e])
+                                   : static_cast<const float*>(t.g[lo])[begin + i + e];
+          mc[h] |= in ? static_cast<uint32_t>(mp[i + e]) << (8 * e) : 0u;
+          uc[h] |= in ? static_cast<uint32_t>(up[i + e]) << (8 * e) : 0u;
+        }
       }
     }
-    m_top = __reduce_max_sync(0xffffffffu, m_top);
-    u_top = __reduce_max_sync(0xffffffffu, u_top);
-  }
-  // Biased exponents of the scales; 1 (2^-126) is the smallest normal one.
-  const int me = max(static_cast<int>(m_top >> 23) - 7, 1);
-  const int ue = max(static_cast<int>(u_top >> 23) - 7, 1);
-  const float m_inv = __uint_as_float(static_cast<unsigned>(254 - me) << 23);
-  const float u_inv = __uint_as_float(static_cast<unsigned>(254 - ue) << 23);
-  if (lane == 0) {
-    t.m_scale[lo][block] = __uint_as_float(static_cast<unsigned>(me) << 23);
-    t.u_scale[lo][block] = __uint_as_float(static_cast<unsigned>(ue) << 23);
-  }
+
+    const float ms = t.m_scale[lo][block], us = t.u_scale[lo][block];
+    float m_max = 0.f, u_max = 0.f;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = h * 128 + lane * 4;
-    float mq[4], uq[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned noise = mix(static_cast<unsigned>(begin + i + e), s.step_mix);
-      const float ma = fabsf(m[h][e]) * m_inv, ua = u[h][e] * u_inv;
-      mq[e] = copysignf(to_grid(ma, noise & 0xffffu), m[h][e]);
-      uq[e] = fmaxf(to_grid(ua, noise >> 16), ua > 0.f ? 0.001953125f : 0.f);
-    }
-    if (spoilt) {
-      const float nan = __uint_as_float(0x7fffffffu);
+    for (int h = 0; h < 2; ++h) {
+      const int i = h * 128 + lane * 4;
+      unpack4(mc[h], m[h]);
+      unpack4(uc[h], u[h]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (magnitude(m[h][e]) >= kInfinity) mq[e] = nan;
-        if (magnitude(u[h][e]) >= kInfinity) uq[e] = nan;
+        const float gi = g[h][e];
+        const float mi = __fadd_rn(__fmul_rn(m[h][e] * ms, s.b1), __fmul_rn(gi, s.c1));
+        const float uo = u[h][e] * us;
+        const float ui = root(__fadd_rn(__fmul_rn(__fmul_rn(uo, uo), s.b2), __fmul_rn(__fmul_rn(gi, gi), s.c2)));
+        w[h][e] = w[h][e] * s.decay - __fdividef(mi * s.step_size, ui + s.eps);
+        m[h][e] = mi;
+        u[h][e] = ui;
+        m_max = largest(m_max, mi);
+        u_max = largest(u_max, ui);
+      }
+      if (whole) {
+        *reinterpret_cast<float4*>(wp + i) = make_float4(w[h][0], w[h][1], w[h][2], w[h][3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (begin + i + e < n) wp[i + e] = w[h][e];
       }
     }
-    const uint32_t mc = pack4(mq), uc = pack4(uq);
-    if (whole) {
-      *reinterpret_cast<float4*>(wp + i) = make_float4(w[h][0], w[h][1], w[h][2], w[h][3]);
-      *reinterpret_cast<uint32_t*>(mp + i) = mc;
-      *reinterpret_cast<uint32_t*>(up + i) = uc;
-    } else {
+    unsigned m_top = warp_top(m_max), u_top = warp_top(u_max);
+    const bool spoilt = max(m_top, u_top) >= kInfinity;  // somewhere in this block
+    if (spoilt) {  // infinities and NaN set no scale
+      m_max = u_max = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (isfinite(m[h][e])) m_max = largest(m_max, m[h][e]);
+          if (isfinite(u[h][e])) u_max = largest(u_max, u[h][e]);
+        }
+      }
+      m_top = warp_top(m_max);
+      u_top = warp_top(u_max);
+    }
+    // Biased exponents of the scales; 1 (2^-126) is the smallest normal one.
+    const int me = max(static_cast<int>(m_top >> 23) - 7, 1);
+    const int ue = max(static_cast<int>(u_top >> 23) - 7, 1);
+    const float m_inv = __uint_as_float(static_cast<unsigned>(254 - me) << 23);
+    const float u_inv = __uint_as_float(static_cast<unsigned>(254 - ue) << 23);
+    if (lane == 0) {
+      t.m_scale[lo][block] = __uint_as_float(static_cast<unsigned>(me) << 23);
+      t.u_scale[lo][block] = __uint_as_float(static_cast<unsigned>(ue) << 23);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = h * 128 + lane * 4;
+      uint32_t mq[4], uq[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (begin + i + e < n) {
-          wp[i + e] = w[h][e];
-          mp[i + e] = static_cast<uint8_t>(mc >> (8 * e));
-          up[i + e] = static_cast<uint8_t>(uc >> (8 * e));
+        const unsigned noise = mix(static_cast<unsigned>(begin + i + e), s.step_mix);
+        mq[e] = to_code(m[h][e] * m_inv, noise & 0xffffu);
+        uq[e] = max(to_code_positive(u[h][e] * u_inv, noise >> 16), min(__float_as_uint(u[h][e]), 1u));
+      }
+      uint32_t m_codes = top_bytes(mq), u_codes = low_bytes(uq);
+      if (spoilt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t byte = 0xffu << (8 * e), nan = 0x7fu << (8 * e);
+          if (!isfinite(m[h][e])) m_codes = (m_codes & ~byte) | nan;
+          if (!isfinite(u[h][e])) u_codes = (u_codes & ~byte) | nan;
+        }
+      }
+      if (whole) {
+        *reinterpret_cast<uint32_t*>(mp + i) = m_codes;
+        *reinterpret_cast<uint32_t*>(up + i) = u_codes;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (begin + i + e < n) {
+            mp[i + e] = static_cast<uint8_t>(m_codes >> (8 * e));
+            up[i + e] = static_cast<uint8_t>(u_codes >> (8 * e));
+          }
         }
       }
     }
@@ -280,9 +298,15 @@ void adamw8_step(const std::vector<torch::Tensor>& weights, const std::vector<to
                 "adamw8: sizes of tensor ", i, " (", n, " weights need ", blocks, " scales of each moment)");
     TORCH_CHECK(blocks < (1ll << 31), "adamw8: tensor ", i, " is too large");
   }
+  // One block a warp while that leaves the launch within what the GPU holds at once, so that a small one is spread over
+  // all of it (3.2 us against 6.9 for 100 thousand elements); else several (1152 us against 1193 for 407 million).
+  unsigned long long all_blocks = 0;
+  for (const auto& w : weights) all_blocks += (w.numel() + kBlock - 1) / kBlock;
+  const int sms = at::cuda::getDeviceProperties(weights[0].get_device())->multiProcessorCount;
   Adam8Batch b;
   unsigned long long ctas = 0;
   b.count = 0;
+  b.rounds = all_blocks > 5ull * sms * kWarps ? kRounds : 1;
   auto flush = [&] {
     if (b.count == 0) return;
     b.first[b.count] = static_cast<unsigned>(ctas);
@@ -295,7 +319,8 @@ void adamw8_step(const std::vector<torch::Tensor>& weights, const std::vector<to
   for (size_t i = 0; i < count; ++i) {
     const int64_t n = weights[i].numel();
     if (n == 0) continue;
-    const unsigned long long need = ((n + kBlock - 1) / kBlock + kWarps - 1) / kWarps;
+    const int64_t per_cta = static_cast<int64_t>(kBlock) * kWarps * b.rounds;
+    const unsigned long long need = (n + per_cta - 1) / per_cta;
     if (b.count == kTensors || ctas + need >= (1ull << 31)) flush();
     const int c = b.count++;
     b.w[c] = weights[i].data_ptr<float>();

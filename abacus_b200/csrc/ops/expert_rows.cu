@@ -14,7 +14,7 @@
 // and sorted rows at or after offsets[E] are zeros (xs, d ys).
 //
 // The sort is a counting sort, stable because every warp takes a contiguous
-// run of assignments and ranks equal experts by lane: one launch up to 2048
+// run of assignments and ranks equal experts by lane: one launch up to 1024
 // assignments, above that one more that counts per part. No atomic decides a
 // place, so results repeat bit for bit.
 //
@@ -37,7 +37,7 @@ namespace {
 constexpr int kMaxExperts = 1024;
 constexpr int kSortWarps = 8;
 constexpr int kSortThreads = kSortWarps * 32;
-constexpr int kPart = 2048;  // assignments of one CTA
+constexpr int kPart = 1024;  // assignments of one CTA
 
 __device__ __forceinline__ int bin_of(const int64_t* indices, long long i, int experts) {
   const int64_t e = indices[i];
@@ -54,10 +54,10 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const int64_t* __re
   for (long long i = begin + threadIdx.x; i < end; i += kSortThreads) atomicAdd(&hist[bin_of(indices, i, experts)], 1);
   __syncthreads();
   for (int e = threadIdx.x; e <= experts; e += kSortThreads)
-    counts[static_cast<long long>(blockIdx.x) * (experts + 1) + e] = hist[e];
+    counts[static_cast<long long>(e) * gridDim.x + blockIdx.x] = hist[e];
 }
 
-// counts: (parts, experts + 1) from count_kernel; unused with one part.
+// counts: (experts + 1, parts) from count_kernel; unused with one part.
 __global__ void __launch_bounds__(kSortThreads) place_kernel(const int64_t* __restrict__ indices, long long n, int experts,
                                                              const int* __restrict__ counts, int* __restrict__ offsets,
                                                              int* __restrict__ order, int* __restrict__ slot) {
@@ -74,23 +74,27 @@ __global__ void __launch_bounds__(kSortThreads) place_kernel(const int64_t* __re
   const long long end = min(begin + kRun, n);
   for (long long i = begin + lane; i < end; i += 32) atomicAdd(&cursor[warp * bins + bin_of(indices, i, experts)], 1);
   __syncthreads();
-  for (int e = threadIdx.x; e < bins; e += kSortThreads) {
+  for (int e = warp; e < bins; e += kSortWarps) {
     int before = 0, all = 0;
     if (parts > 1) {
-#pragma unroll 8
-      for (int p = 0; p < parts; ++p) {
-        const int c = counts[static_cast<long long>(p) * bins + e];
+      for (int p = lane; p < parts; p += 32) {
+        const int c = counts[static_cast<long long>(e) * parts + p];
         all += c;
         before += p < static_cast<int>(blockIdx.x) ? c : 0;
       }
+      all = __reduce_add_sync(0xffffffffu, all);
+      before = __reduce_add_sync(0xffffffffu, before);
     }
-    int run = before;
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = cursor[w * bins + e];
-      cursor[w * bins + e] = run;
-      run += c;
+    // Lane w: where warp w's assignments to this bin start.
+    const int mine = lane < kSortWarps ? cursor[lane * bins + e] : 0;
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < kSortWarps; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
     }
-    start[e] = parts > 1 ? all : run;
+    if (lane < kSortWarps) cursor[lane * bins + e] = before + sum - mine;
+    if (lane == kSortWarps - 1) start[e] = parts > 1 ? all : sum;
   }
   __syncthreads();
   if (warp == 0) {  // exclusive sum over the bins
@@ -216,7 +220,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ ys, 
   }
 }
 
-template <class T, int N>
+// GROUP choices of a token at a time, so that d out[t] is read once for them: two where the number of choices is even
+// (90 us against 95 one at a time for 65536 tokens, 2 choices, 768 bf16), one where it is odd (40 us against 51 two at a
+// time for 9001 tokens, 3 choices, 770 fp32).
+template <class T, int N, int GROUP>
 __global__ void __launch_bounds__(256) combine_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ ys,
                                                           const float* __restrict__ weights, const int* __restrict__ slot,
                                                           const int* __restrict__ end, T* __restrict__ dys,
@@ -228,29 +235,45 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const T* __restrict__ 
   const long long count = tokens * choices;
   for (long long t = warp; t < tokens; t += warps) {
     const Pack<T, N>* d = reinterpret_cast<const Pack<T, N>*>(dout) + t * packs;
-    for (int k = 0; k < choices; ++k) {  // d out[t] stays in the L1 cache over k
-      const long long s = slot[t * choices + k];
-      float dot = 0.f;
-      if (s >= 0 && s < count) {
-        const float w = weights[t * choices + k];
-        const Pack<T, N>* y = reinterpret_cast<const Pack<T, N>*>(ys) + s * packs;
-        Pack<T, N>* dy = reinterpret_cast<Pack<T, N>*>(dys) + s * packs;
+    for (int k = 0; k < choices; k += GROUP) {
+      long long s[GROUP];
+      float w[GROUP], dot[GROUP];
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i) {
+        const long long r = slot[t * choices + k + i];
+        s[i] = r < count ? r : -1;
+        w[i] = weights[t * choices + k + i];
+        dot[i] = 0.f;
+      }
 #pragma unroll 2
-        for (long long c = lane; c < packs; c += 32) {
-          const Pack<T, N> a = d[c], b = y[c];
+      for (long long c = lane; c < packs; c += 32) {
+        const Pack<T, N> a = d[c];
+        Pack<T, N> y[GROUP];
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i)
+          if (s[i] >= 0) y[i] = reinterpret_cast<const Pack<T, N>*>(ys)[s[i] * packs + c];
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) {
+          if (s[i] < 0) continue;
           Pack<T, N> o;
 #pragma unroll
           for (int e = 0; e < N; ++e) {
             const float g = to_float(a.v[e]);
-            dot = fmaf(g, to_float(b.v[e]), dot);
-            o.v[e] = from_float<T>(w * g);
+            dot[i] = fmaf(g, to_float(y[i].v[e]), dot[i]);
+            o.v[e] = from_float<T>(w[i] * g);
           }
-          dy[c] = o;
+          reinterpret_cast<Pack<T, N>*>(dys)[s[i] * packs + c] = o;
         }
       }
 #pragma unroll
-      for (int m = 16; m > 0; m /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, m);
-      if (lane == 0) dweights[t * choices + k] = dot;
+      for (int m = 16; m > 0; m /= 2) {
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], m);
+      }
+      if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) dweights[t * choices + k + i] = dot[i];
+      }
     }
   }
   zero_tail<T, N>(dys, count, end, packs, warp, warps, lane);
@@ -409,7 +432,8 @@ void expert_combine_bwd(torch::Tensor dout, torch::Tensor ys, torch::Tensor weig
   with_pack(ys, pack_of(dim, dim, element, {ys.data_ptr(), dout.data_ptr(), dys.data_ptr()}), [&](auto zero, auto n) {
     using T = decltype(zero);
     constexpr int N = decltype(n)::value;
-    combine_bwd_kernel<T, N><<<row_blocks(tokens, ys), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+    const auto kernel = choices % 2 == 0 ? combine_bwd_kernel<T, N, 2> : combine_bwd_kernel<T, N, 1>;
+    kernel<<<row_blocks(tokens, ys), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
         static_cast<const T*>(dout.data_ptr()), static_cast<const T*>(ys.data_ptr()), weights.data_ptr<float>(),
         slot.data_ptr<int>(), end, static_cast<T*>(dys.data_ptr()), dweights.data_ptr<float>(), tokens,
         static_cast<int>(choices), dim / N);
