@@ -32,6 +32,13 @@ combine is a weighted ``index_add`` in sorted order (deterministic). With a
 capacity factor (CUDA), every expert owns a static slab of C rows and all
 experts run as one grouped launch per product (``gemm.grouped_swiglu_mlp``),
 with no host sync.
+
+``MoE(ragged=True)`` runs the dropless operators of ``ops/experts.py`` instead:
+the plan, the gather, the experts over ragged row counts and the combine stay on
+the device and no row is padded; with a capacity factor the assignments past an
+expert's capacity are dropped from the plan. ``expert_dtype=torch.bfloat16``
+casts the rows and the experts' matrices for those products (parameters, router
+and combine weights stay fp32).
 """
 from __future__ import annotations
 
@@ -40,7 +47,7 @@ import os
 
 import torch
 
-from abacus_b200.ops import gemm
+from abacus_b200.ops import experts, gemm
 from abacus_b200.ops._ext import ext
 from abacus_b200.ops.routing import expert_rank
 from abacus_b200.parallel import ep_fused, mesh, tp_fused
@@ -295,6 +302,8 @@ class MoE(torch.nn.Module):
         router: str = "sigmoid",
         capacity_factor: float | None = None,
         aux_loss_coeff: float = 1e-2,
+        ragged: bool = False,
+        expert_dtype: torch.dtype | None = None,
     ):
         super().__init__()
         self.dim = dim
@@ -304,6 +313,12 @@ class MoE(torch.nn.Module):
         self.capacity_factor = capacity_factor
         if self.hidden_dim < 1:
             raise ValueError(f"hidden_dim must be at least 1, got {self.hidden_dim}")
+        if expert_dtype not in (None, torch.float32, torch.bfloat16):
+            raise ValueError(f"expert_dtype must be float32 or bfloat16, got {expert_dtype}")
+        if expert_dtype is not None and not ragged:
+            raise ValueError("expert_dtype needs ragged=True")
+        self.ragged = ragged
+        self.expert_dtype = expert_dtype
         self.router = Router(
             dim, n_experts, top_k, bias_update_speed=bias_update_speed, route_scale=route_scale,
             router=router, aux_loss_coeff=aux_loss_coeff,
@@ -336,12 +351,24 @@ class MoE(torch.nn.Module):
         if x_TD.shape[0] == 0:
             return x_BLD
         capacity = self._capacity(x_TD.shape[0])
-        if capacity is not None and x_TD.is_cuda:
+        if getattr(self, "ragged", False):
+            out_TD = self._ragged_experts(x_TD, weights_TK, indices_TK, capacity)
+        elif capacity is not None and x_TD.is_cuda:
             out_TD = _grouped_experts_capacity(x_TD, weights_TK, indices_TK, self.w_gate_EDM, self.w_up_EDM,
                                                self.w_down_EMD, capacity)
         else:
             out_TD = _grouped_experts(x_TD, weights_TK, indices_TK, self.w_gate_EDM, self.w_up_EDM, self.w_down_EMD)
         return out_TD.reshape(batch, length, self.dim)
+
+    def _ragged_experts(self, x_TD, weights_TK, indices_TK, capacity):
+        if capacity is not None:
+            indices_TK = torch.where(_capacity_keep(indices_TK, self.n_experts, capacity), indices_TK, -1)
+        plan = experts.expert_plan(indices_TK, self.n_experts)
+        dtype = x_TD.dtype if self.expert_dtype is None else self.expert_dtype
+        xs_SD = experts.dispatch_tokens(x_TD.to(dtype), plan)
+        ys_SD = experts.ragged_swiglu_mlp(xs_SD, self.w_gate_EDM.to(dtype), self.w_up_EDM.to(dtype),
+                                          self.w_down_EMD.to(dtype), plan.offsets)
+        return experts.combine_tokens(ys_SD, weights_TK.float(), plan).to(x_TD.dtype)
 
     def _capacity(self, tokens: int) -> int | None:
         """Per-expert capacity of this rank's tokens (None without a capacity factor)."""

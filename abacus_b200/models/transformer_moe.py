@@ -4,7 +4,7 @@
 Attention is never tensor parallel here; expert parallelism forbids dropout
 because every rank must keep identical replicated activations. Options beyond
 the reference (router type, capacity factor, aux-loss coefficient, EP over
-data-parallel ranks) default to the reference's behaviour.
+data-parallel ranks, ragged experts and their type) default to the reference's behaviour.
 """
 from __future__ import annotations
 
@@ -34,6 +34,8 @@ class TransformerBlockMoe(torch.nn.Module):
         capacity_factor: float | None = None,
         aux_loss_coeff: float = 1e-2,
         expert_data_parallel: bool = False,
+        ragged: bool = False,
+        expert_dtype: torch.dtype | None = None,
     ):
         super().__init__()
         _, world_size = mesh.rank_and_world_size("ep")
@@ -49,10 +51,12 @@ class TransformerBlockMoe(torch.nn.Module):
             hidden_dim=hidden_dim, bias_update_speed=bias_update_speed, route_scale=route_scale, router=router,
             capacity_factor=capacity_factor, aux_loss_coeff=aux_loss_coeff,
         )
+        if expert_parallel and ragged:
+            raise ValueError("ragged experts do not combine with expert parallel")
         if expert_parallel:
             self.moe = MoEExpertParallel(dim, n_experts, top_k, data_parallel=expert_data_parallel, **kwargs)
         else:
-            self.moe = MoE(dim, n_experts, top_k, **kwargs)
+            self.moe = MoE(dim, n_experts, top_k, ragged=ragged, expert_dtype=expert_dtype, **kwargs)
         self.dropout = torch.nn.Dropout(dropout)
 
     def forward(self, x_BLD: torch.Tensor, rotary: torch.nn.Module | None = None) -> torch.Tensor:
@@ -83,6 +87,8 @@ class TransformerMoe(torch.nn.Module):
         aux_loss_coeff: float = 1e-2,
         expert_data_parallel: bool = False,
         init_std: float = 1.0,
+        ragged: bool = False,
+        expert_dtype: torch.dtype | None = None,
     ):
         super().__init__()
         self.dim = dim
@@ -102,7 +108,7 @@ class TransformerMoe(torch.nn.Module):
                     dim, n_heads, head_dim, n_experts, top_k, dropout, hidden_dim=hidden_dim,
                     bias_update_speed=bias_update_speed, route_scale=route_scale, expert_parallel=expert_parallel,
                     router=router, capacity_factor=capacity_factor, aux_loss_coeff=aux_loss_coeff,
-                    expert_data_parallel=expert_data_parallel,
+                    expert_data_parallel=expert_data_parallel, ragged=ragged, expert_dtype=expert_dtype,
                 )
                 for _ in range(n_blocks)
             ]

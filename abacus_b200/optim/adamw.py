@@ -14,15 +14,24 @@ ZeRO (moments are allocated for exactly that range up front), ``grad_shards``
 holds the already-reduced gradient of that range (ZeRO-2/3), and the state of
 a parameter is ``{"step", "exp_avg", "exp_avg_sq"}`` keyed by ``id(param)``.
 
+With ``state_bits=8`` both moments are held in 8 bits (``ops/adamw8.py``): the
+state of a parameter is ``{"step", "exp_avg", "exp_avg_scale", "exp_rms",
+"exp_rms_scale"}``, 2.03 bytes an element in place of 8. Weights must be fp32;
+gradients may be bf16. Checkpoints hold 32-bit moments either way, so a run can
+go on with the other width. It does not combine with the fused data-parallel
+optimizers, which keep their own 32-bit moments.
+
 Execution: parameters are grouped by (device, step count). On CUDA each group
 is one multi-tensor kernel launch per 36 tensors (``csrc/ops/embed_ce_adamw.cu``);
 elsewhere each group runs the same update as ``torch._foreach_*`` operations,
-which apply the formulas above element by element in the order written.
+which apply the formulas above element by element in the order written. 8-bit
+groups are one launch per 128 tensors (``csrc/ops/adamw8.cu``).
 """
 from __future__ import annotations
 
 import torch
 
+from abacus_b200.ops import adamw8
 from abacus_b200.ops._ext import ext
 
 _NOT_OWNED = object()
@@ -52,7 +61,10 @@ class AdamW:
         weight_decay: float = 1e-2,
         owned: dict[int, tuple[int, int]] | None = None,
         grad_shards: dict[int, torch.Tensor] | None = None,
+        state_bits: int = 32,
     ):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits!r}")
         _check_hyperparameters(lr, betas, eps, weight_decay)
         self.params = list(model.parameters()) if isinstance(model, torch.nn.Module) else list(model)
         self.lr = lr
@@ -61,14 +73,18 @@ class AdamW:
         self.weight_decay = weight_decay
         self.owned = owned
         self.grad_shards = grad_shards
+        self.state_bits = state_bits
         self.state: dict[int, dict[str, torch.Tensor | int]] = {}
         for param in self.params if owned is not None else ():
             span = owned.get(id(param))
             if span is not None:
                 self.state[id(param)] = self._fresh_state(span[1] - span[0], param)
 
-    @staticmethod
-    def _fresh_state(numel: int, like: torch.Tensor) -> dict:
+    def _fresh_state(self, numel: int, like: torch.Tensor) -> dict:
+        if self.state_bits == 8:
+            if like.dtype != torch.float32:
+                raise ValueError(f"AdamW: 8-bit moments need fp32 weights, got {like.dtype}")
+            return {"step": 0, **adamw8.fresh_state(numel, like.device)}
         zeros = lambda: torch.zeros(numel, dtype=like.dtype, device=like.device)  # noqa: E731
         return {"step": 0, "exp_avg": zeros(), "exp_avg_sq": zeros()}
 
@@ -127,14 +143,30 @@ class AdamW:
             state = self.state.get(id(param))
             if state is None:
                 state = self.state[id(param)] = self._fresh_state(weight.numel(), weight)
-            if state["exp_avg"].shape != weight.shape:  # flat moments of a whole parameter
+            if self.state_bits == 32 and state["exp_avg"].shape != weight.shape:  # flat moments of a whole parameter
                 state["exp_avg"] = state["exp_avg"].view(weight.shape)
                 state["exp_avg_sq"] = state["exp_avg_sq"].view(weight.shape)
             state["step"] += 1
             key = (weight.device, state["step"], weight.is_cuda and weight.dtype == torch.float32)
             groups.setdefault(key, []).append((weight, grad, state))
         for (_, step, on_kernel), items in groups.items():
-            (self._launch_kernel if on_kernel else self._foreach_update)(items, step)
+            if self.state_bits == 8:
+                self._step_8_bit(items, step)
+            else:
+                (self._launch_kernel if on_kernel else self._foreach_update)(items, step)
+
+    def _step_8_bit(self, items, step: int) -> None:
+        weights = [w if w.is_contiguous() else w.contiguous() for w, _, _ in items]
+        grads = [g if g.dtype in (torch.float32, torch.bfloat16) else g.float() for _, g, _ in items]
+        states = [s for _, _, s in items]
+        adamw8.step_(
+            weights, [g.contiguous() for g in grads],
+            *([s[key] for s in states] for key in ("exp_avg", "exp_avg_scale", "exp_rms", "exp_rms_scale")),
+            lr=self.lr, betas=(self.beta1, self.beta2), eps=self.eps, weight_decay=self.weight_decay, step=step,
+        )
+        for (w, _, _), wc in zip(items, weights):
+            if wc is not w:
+                w.copy_(wc)
 
     def _launch_kernel(self, items, step: int) -> None:
         weights = [w if w.is_contiguous() else w.contiguous() for w, _, _ in items]
@@ -167,15 +199,36 @@ class AdamW:
         torch._foreach_addcdiv_(weights, m, denom, value=-(self.lr / correction1))
 
     # ------------------------------------------------------------ checkpoints
+    def moments(self, state: dict) -> dict[str, torch.Tensor]:
+        """``{"exp_avg", "exp_avg_sq"}`` of a parameter's state in 32 bits."""
+        if "exp_rms" not in state:
+            return {key: state[key] for key in ("exp_avg", "exp_avg_sq")}
+        return {"exp_avg": adamw8.dequantize(state["exp_avg"], state["exp_avg_scale"]),
+                "exp_avg_sq": adamw8.dequantize(state["exp_rms"], state["exp_rms_scale"]) ** 2}
+
     def state_dict_by_name(self, model: torch.nn.Module) -> dict:
-        """Optimizer state keyed by parameter name (for checkpoints)."""
-        named = ((name, self.state.get(id(p))) for name, p in model.named_parameters())
-        return {name: {k: st[k] for k in ("step", "exp_avg", "exp_avg_sq")} for name, st in named if st is not None}
+        """Optimizer state keyed by parameter name (for checkpoints), in 32 bits."""
+        named = ((name, p, self.state.get(id(p))) for name, p in model.named_parameters())
+        out = {}
+        for name, p, st in named:
+            if st is not None:
+                moments = self.moments(st)
+                if "exp_rms" in st and st["exp_avg"].numel() == p.numel():
+                    moments = {key: t.view(p.shape) for key, t in moments.items()}
+                out[name] = {"step": st["step"], **moments}
+        return out
 
     def load_state_dict_by_name(self, model: torch.nn.Module, state: dict) -> None:
         for name, param in model.named_parameters():
             saved = state.get(name)
             if saved is None:
+                continue
+            if self.state_bits == 8:
+                state = self.state[id(param)] = self._fresh_state(0, param)
+                state["step"] = int(saved["step"])
+                m, v = (saved[key].to(device=param.device, dtype=torch.float32) for key in ("exp_avg", "exp_avg_sq"))
+                state["exp_avg"], state["exp_avg_scale"] = adamw8.quantize(m)
+                state["exp_rms"], state["exp_rms_scale"] = adamw8.quantize(v.sqrt(), positive=True)
                 continue
             self.state[id(param)] = {
                 "step": int(saved["step"]),

@@ -15,6 +15,7 @@ Differences from the reference, none of which change the maths:
   tensors.
 * Optional optimizer / schedule hyper-parameters (the reference hard-codes
   AdamW's defaults and ``WSD(total_steps)``); defaults are the reference's.
+  ``state_bits=8`` holds AdamW's moments in 8 bits.
 * MoE models with the softmax router add their load-balancing loss.
 * Pipeline and context parallel may be combined through a mesh (the
   reference forbids PP + CP).
@@ -65,6 +66,7 @@ class Trainer:
         print_memory: bool = False,
         device: torch.device | str | None = None,
         tracer: PhaseTracer | None = None,
+        state_bits: int = 32,
     ):
         if parallel is not None and pipeline is not None and mesh.get_mesh() is None:
             raise ValueError("pipeline parallel does not use DataParallel")
@@ -84,9 +86,11 @@ class Trainer:
             grad_shards = parallel.grad_shards
         self.optimizer = AdamW(
             self.model, lr=1e-3 if lr is None else lr, betas=betas, eps=eps, weight_decay=weight_decay,
-            owned=owned, grad_shards=grad_shards,
+            owned=owned, grad_shards=grad_shards, state_bits=state_bits,
         )
         self._fused = bool(getattr(parallel, "fused_optimizer", False))
+        if self._fused and state_bits != 32:
+            raise ValueError("the fused data-parallel optimizers keep 32-bit moments")
         if self._fused and pipeline is not None:
             raise ValueError("the fused data-parallel optimizer does not combine with pipeline parallel")
         if self._fused:

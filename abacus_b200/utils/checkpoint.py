@@ -103,8 +103,9 @@ def full_optimizer_state(model, optimizer, parallel=None) -> dict[str, dict]:
         dist.all_reduce(t, op=dist.ReduceOp.MAX, group=parallel.group)
         step = int(t.item())
     moments = {}
+    local = {pid: optimizer.moments(st) for pid, st in states.items() if st is not None}
     for key in ("exp_avg", "exp_avg_sq"):
-        pieces = {pid: st[key] for pid, st in states.items() if st is not None}
+        pieces = {pid: st[key] for pid, st in local.items()}
         if owned is not None:
             # ZeRO-sharded moments: every rank holds only its owned range.
             gathered = parallel.gather_owned(pieces)
