@@ -46,7 +46,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("expert_combine", &abacus::experts::combine, "weighted sum of each token's expert rows (differentiable)");
   m.def("ragged_matmul", &abacus::experts::matmul, "sorted rows times their experts' matrices (differentiable)");
   m.def("ragged_swiglu_mlp", &abacus::experts::swiglu_mlp, "SwiGLU experts over sorted rows (differentiable)");
-  m.def("ragged_stage", &abacus::ragged::stage, "bf16 planes of an operand of the ragged products");
+  m.def("ragged_stage", &abacus::ragged::stage, "bf16 planes of an operand of the ragged products",
+        py::arg("t"), py::arg("planes"), py::arg("offsets") = py::none());
   m.def("ragged_rows", &abacus::ragged::rows, "sorted rows times their experts' matrices, staged operands");
   m.def("ragged_swiglu", &abacus::ragged::swiglu, "gate and up products with the SwiGLU epilogue, staged operands");
   m.def("ragged_swiglu_bwd", &abacus::ragged::swiglu_bwd, "gradient through the down product with the SwiGLU derivative");

@@ -6,7 +6,7 @@
 
 namespace abacus {
 namespace ragged {
-torch::Tensor stage(torch::Tensor t, int64_t planes);
+torch::Tensor stage(torch::Tensor t, int64_t planes, c10::optional<torch::Tensor> offsets);
 void rows(std::vector<torch::Tensor> a, std::vector<torch::Tensor> b, torch::Tensor offsets, torch::Tensor out,
           bool transposed);
 void swiglu(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, torch::Tensor offsets, torch::Tensor g,

@@ -74,15 +74,15 @@ struct Combine : torch::autograd::Function<Combine> {
 };
 
 // `t` as the product kernels read it: bf16 planes first, rows 16-byte aligned. bf16 tensors laid out so already are used in
-// place.
-Tensor operand(const Tensor& t, int64_t planes) {
+// place. With offsets, `t` holds the experts' matrices, and those of experts without rows are left out of a copy.
+Tensor operand(const Tensor& t, int64_t planes, c10::optional<Tensor> offsets = c10::nullopt) {
   const int64_t d = t.dim();
   if (t.scalar_type() == torch::kBFloat16 && t.stride(d - 1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) {
     bool aligned = t.size(d - 2) <= 1 || t.stride(d - 2) >= t.size(d - 1);
     for (int64_t i = 0; i < d - 1; ++i) aligned = aligned && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) > 0));
     if (aligned) return t.unsqueeze(0);
   }
-  return ragged::stage(t, planes);
+  return ragged::stage(t, planes, offsets);
 }
 
 Tensor like_matrix(const Tensor& w) { return torch::empty(w.sizes(), w.options()); }
@@ -96,10 +96,13 @@ Tensor padded(int64_t planes, int64_t rows, int64_t cols, torch::TensorOptions o
 
 struct RaggedMatmul : torch::autograd::Function<RaggedMatmul> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t planes) {
-    ctx->save_for_backward({x, w, offsets});
+    // The backward reads x as an operand: where that is a copy it is kept in place of x (6 bytes an element in fp32; w's,
+    // which would stay for the whole forward of a model, is made again).
+    const auto xo = operand(x, planes);
+    ctx->save_for_backward({xo, w, offsets});
     ctx->saved_data["planes"] = planes;
     auto y = torch::empty({x.size(0), w.size(2)}, x.options());
-    ragged::rows({operand(x, planes)}, {operand(w, planes)}, offsets, y, false);
+    ragged::rows({xo}, {operand(w, planes, offsets)}, offsets, y, false);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -110,12 +113,12 @@ struct RaggedMatmul : torch::autograd::Function<RaggedMatmul> {
     const auto dy = operand(grads[0], planes);
     Tensor dx, dw;
     if (ctx->needs_input_grad(0)) {
-      dx = torch::empty(x.sizes(), x.options());
-      ragged::rows({dy}, {operand(w, planes)}, offsets, dx, true);
+      dx = torch::empty({x.size(1), x.size(2)}, w.options());
+      ragged::rows({dy}, {operand(w, planes, offsets)}, offsets, dx, true);
     }
     if (ctx->needs_input_grad(1)) {
       dw = like_matrix(w);
-      ragged::weights(operand(x, planes), {dy}, offsets, {dw});
+      ragged::weights(x, {dy}, offsets, {dw});
     }
     return {dx, dw, Tensor(), Tensor()};
   }
@@ -127,12 +130,13 @@ struct RaggedSwiGLU : torch::autograd::Function<RaggedSwiGLU> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
                         const Tensor& w_down, const Tensor& offsets, int64_t planes) {
     const int64_t rows = x.size(0), hidden = w_gate.size(2);
-    const auto g = padded(0, rows, hidden, x.options()), u = padded(0, rows, hidden, x.options());
+    const auto kept = x.options().dtype(torch::kFloat32);
+    const auto g = padded(0, rows, hidden, kept), u = padded(0, rows, hidden, kept);
     const auto h = padded(planes, rows, hidden, x.options().dtype(torch::kBFloat16));
     auto y = torch::empty({rows, w_down.size(2)}, x.options());
     const auto xo = operand(x, planes);
-    ragged::swiglu(xo, operand(w_gate, planes), operand(w_up, planes), offsets, g, u, h);
-    ragged::rows({h}, {operand(w_down, planes)}, offsets, y, false);
+    ragged::swiglu(xo, operand(w_gate, planes, offsets), operand(w_up, planes, offsets), offsets, g, u, h);
+    ragged::rows({h}, {operand(w_down, planes, offsets)}, offsets, y, false);
     ctx->save_for_backward({xo, w_gate, w_up, w_down, offsets, g, u, h});
     return y;
   }
@@ -144,11 +148,11 @@ struct RaggedSwiGLU : torch::autograd::Function<RaggedSwiGLU> {
     const int64_t planes = h.size(0), rows = g.size(0), hidden = g.size(1);
     const auto dy = operand(grads[0], planes);
     const auto dg = padded(planes, rows, hidden, h.options()), du = padded(planes, rows, hidden, h.options());
-    ragged::swiglu_bwd(dy, operand(w_down, planes), offsets, g, u, dg, du);
+    ragged::swiglu_bwd(dy, operand(w_down, planes, offsets), offsets, g, u, dg, du);
     variable_list out(6);
     if (ctx->needs_input_grad(0)) {
-      out[0] = torch::empty({rows, x.size(2)}, g.options());
-      ragged::rows({dg, du}, {operand(w_gate, planes), operand(w_up, planes)}, offsets, out[0], true);
+      out[0] = torch::empty({rows, x.size(2)}, w_gate.options());
+      ragged::rows({dg, du}, {operand(w_gate, planes, offsets), operand(w_up, planes, offsets)}, offsets, out[0], true);
     }
     if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
       Tensor dw_gate = like_matrix(w_gate), dw_up = like_matrix(w_up);

@@ -67,6 +67,7 @@ struct StageParams {
   long long batch, rows, cols, ld;
   int planes;
   void* dst;
+  const int* offsets;  // batch + 1 row offsets (may be null): matrices whose expert has no rows are left out
 };
 cudaError_t launch_stage(const StageParams& p, int sms, cudaStream_t stream);
 

@@ -68,13 +68,12 @@ void check_result(const torch::Tensor& t, const torch::Tensor& like, int64_t pla
               name, " must be a contiguous ", planes == 1 ? "bf16" : "fp32", " tensor of shape ", shape);
 }
 
-// Rows that a SwiGLU form keeps for itself: (rows, cols) with rows padded to 16 bytes.
-void check_kept(const torch::Tensor& t, const torch::Tensor& like, int64_t planes, int64_t rows, int64_t cols, const char* name) {
+// Rows that a SwiGLU form keeps for itself: fp32 (rows, cols) with rows padded to 16 bytes.
+void check_kept(const torch::Tensor& t, const torch::Tensor& like, int64_t rows, int64_t cols, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols &&
-                  t.scalar_type() == (planes == 1 ? torch::kBFloat16 : torch::kFloat32) && t.stride(1) == 1 &&
-                  t.stride(0) * t.element_size() % 16 == 0 && t.stride(0) >= (cols * t.element_size() + 15) / 16 * 16 / t.element_size() &&
-                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              name, " must have 16-byte aligned rows");
+                  t.scalar_type() == torch::kFloat32 && t.stride(1) == 1 && t.stride(0) % 4 == 0 &&
+                  t.stride(0) >= (cols + 3) / 4 * 4 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              name, " must be fp32 with 16-byte aligned rows");
 }
 
 // An operand that a SwiGLU form writes: (planes, rows, cols) with padded rows.
@@ -132,7 +131,7 @@ void check_rows_and_matrices(const torch::Tensor& a, const torch::Tensor& b, int
 
 }  // namespace
 
-torch::Tensor stage(torch::Tensor t, int64_t planes) {
+torch::Tensor stage(torch::Tensor t, int64_t planes, c10::optional<torch::Tensor> offsets) {
   const c10::cuda::CUDAGuard guard(t.device());
   TORCH_CHECK(t.is_cuda() && (t.dim() == 2 || t.dim() == 3), "stage takes 2-D or 3-D CUDA tensors");
   const bool bf16 = t.scalar_type() == torch::kBFloat16;
@@ -154,6 +153,13 @@ torch::Tensor stage(torch::Tensor t, int64_t planes) {
   p.ld = ld;
   p.planes = static_cast<int>(planes);
   p.dst = out.data_ptr();
+  p.offsets = nullptr;
+  if (offsets) {
+    TORCH_CHECK(batched && offsets->is_cuda() && offsets->scalar_type() == torch::kInt32 && offsets->is_contiguous() &&
+                    offsets->numel() == batch + 1,
+                "offsets of the experts' matrices");
+    p.offsets = offsets->data_ptr<int>();
+  }
   C10_CUDA_CHECK(launch_stage(p, sms_of(t), at::cuda::getCurrentCUDAStream()));
   host::note_launch();
   return out.narrow(-1, 0, cols);
@@ -200,7 +206,7 @@ void swiglu(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, torch::Te
     check_rows_and_matrices(x, w, p.experts, k, "the experts' matrices");
     TORCH_CHECK(w.size(2) == k && w.size(3) == n, "ragged SwiGLU shapes");
   }
-  for (const auto& t : {g, u}) check_kept(t, x, planes, s, n, "gate and up");
+  for (const auto& t : {g, u}) check_kept(t, x, s, n, "gate and up");
   check_written(h, x, planes, s, n, "their product");
   if (s == 0 || n == 0) return;
   TORCH_CHECK(k > 0, "empty contraction");
@@ -228,7 +234,7 @@ void swiglu_bwd(torch::Tensor dy, torch::Tensor w_down, torch::Tensor offsets, t
   Params p = params_of(offsets, dy, s);
   check_rows_and_matrices(dy, w_down, p.experts, k, "the down matrices");
   TORCH_CHECK(w_down.size(2) == n && w_down.size(3) == k, "ragged SwiGLU backward shapes");
-  for (const auto& t : {g, u}) check_kept(t, dy, planes, s, n, "gate and up");
+  for (const auto& t : {g, u}) check_kept(t, dy, s, n, "gate and up");
   for (const auto& t : {dg, du}) check_written(t, dy, planes, s, n, "the gradients of gate and up");
   TORCH_CHECK(g.stride(0) == u.stride(0), "gate and up must have one row stride");
   if (s == 0 || n == 0) return;

@@ -40,6 +40,8 @@ constexpr int kThreads = 384;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
 constexpr int kStageOutBytes = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes
 
+constexpr bool split_registers(int planes, Epilogue epi) { return planes > 1 || epi == kSwiGLUBwd; }
+
 template <int PLANES, bool PAIR>
 struct Config {
   static constexpr int kBN = tile_cols(PAIR);
@@ -50,8 +52,9 @@ struct Config {
   static constexpr int kStages = 6 / PLANES;  // 192 KB of stages
   static constexpr uint32_t kTmemCols = 2 * kBN;
   static constexpr int kTableBytes = (kMaxExperts + 2) * 4;
-  // Register split with several planes, whose epilogue threads hold half a row of fp32 sums: 128 x 72 + 256 x 216 is
-  // what 384 threads are launched with (168 each).
+  // Register split of the kernels whose epilogue threads hold half a row of fp32 sums (several planes) or 32 columns of g
+  // and u ahead (SwiGLU backward): 128 x 72 + 256 x 216 is what 384 threads are launched with (168 each; the launcher
+  // checks that).
   static constexpr uint32_t kRegsControl = 72, kRegsEpilogue = 216;
   static_assert(128 * kRegsControl + 256 * kRegsEpilogue <= kThreads * 168, "register split above the launch's total");
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kStageOutBytes + kTableBytes;
@@ -221,16 +224,23 @@ struct Rows32 {
 
 };
 
-// The SwiGLU epilogues work on 64 bytes of a row of g and u at a time.
+// Columns that the SwiGLU epilogues work on at a time: 64 bytes of a row of a result's type.
 template <class Out>
 constexpr int kSpan = 64 / static_cast<int>(sizeof(Out));
 
-// A warp's 32 rows of one bf16 span, in the order of whole rows: lane / 4 and a quarter of the row each.
-struct Span {
-  uint4 v[4];
-  __device__ void load_quarter(int i, int lane, const __nv_bfloat16* base, long long ld, int rows, int col0, int cols) {
+// A quarter of a warp's 32 rows of 32 fp32 columns, in the order of whole rows: 8 columns of row 8 i + lane / 4.
+struct Quarter {
+  uint4 v[2];
+  __device__ void load(int i, int lane, const float* base, long long ld, int rows, int col0, int cols) {
     const int col = col0 + (lane % 4) * 8, r = i * 8 + lane / 4;
-    v[i] = r < rows && col < cols ? *reinterpret_cast<const uint4*>(base + r * ld + col) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      v[j] = r < rows && col + 4 * j < cols ? *reinterpret_cast<const uint4*>(base + r * ld + col + 4 * j)
+                                            : make_uint4(0, 0, 0, 0);
+  }
+  __device__ void get(float (&x)[8]) const {
+    OutTraits<float>::unpack(v[0], x);
+    OutTraits<float>::unpack(v[1], x + 4);
   }
 };
 
@@ -250,6 +260,15 @@ __device__ __forceinline__ void store_span(uint8_t* staging, int lane, Out* base
     if (r < rows && col < cols)
       *reinterpret_cast<uint4*>(base + r * ld + col) = *reinterpret_cast<const uint4*>(staging + unit_at<4>(r, lane % 4));
   }
+}
+
+// Stores columns of g or u, which are fp32 with padded rows whatever the results' type: rounded to bf16 they would put
+// as much error into the gradients as the rounding of those does (3.1e-3 of the gradients' norm against 2.4e-3).
+template <int COLS>
+__device__ __forceinline__ void store_kept(uint8_t* staging, int lane, float* base, long long ld, int rows, int col0, int cols,
+                                           const float (&v)[COLS]) {
+  if constexpr (COLS == 32) Rows32<float>::store(staging, lane, base, ld, rows, col0, cols, true, v);
+  else store_span<float>(staging, lane, base, ld, rows, col0, cols, v);
 }
 
 // Stores a span as an operand of the next product: with one plane the bf16 numbers themselves, else their parts (16
@@ -297,6 +316,7 @@ struct Tile {
   int steps;      // stages of the contraction
   int k_row0;     // weights: first sorted row of the contraction
   int k_rows;     // weights: their number
+  bool narrow;    // the output ends in the first half of the tile's columns, and only they are made
 };
 
 template <int PLANES, bool PAIR, bool WEIGHTS, bool B_MN, Epilogue EPI>
@@ -409,11 +429,14 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       t.k_row0 = t.k_rows = 0;
       t.steps = e == p.experts ? 0 : p.segments * steps_per_segment;
     }
+    // (A single CTA's 128 columns stay whole, and the gate and up halves of a SwiGLU tile are both needed.)
+    t.narrow = PAIR && EPI != kSwiGLU && p.n - t.n0 <= Cfg::kBN / 2;
     return t;
   };
 
+  constexpr bool kSplit = split_registers(PLANES, EPI);
   if (warp < kEpiWarp0) {
-    if constexpr (PLANES > 1) regs_decrease<Cfg::kRegsControl>();
+    if constexpr (kSplit) regs_decrease<Cfg::kRegsControl>();
   }
   if (warp == 0) {
     // -------------------------------------------------------------- loads
@@ -437,15 +460,19 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
           const int k0 = k_next;
           k_next += kDepth;
           const bool tail = WEIGHTS && (step + 1) * kDepth > t.k_rows;
+          const uint32_t bytes = Cfg::kStageBytes - (B_MN && t.narrow ? PLANES * Cfg::kBBytes / 2 : 0);
           uint32_t bar;
           if (tail) {
             bar = smem_u32(&tail_bar[s]);
-            mbar_arrive_expect_tx(&tail_bar[s], Cfg::kStageBytes);
+            mbar_arrive_expect_tx(&tail_bar[s], bytes);
           } else {
             bar = leader_addr(&full_bar[s]);
-            if (PAIR) arrive_expect_cluster(bar, Cfg::kStageBytes);
-            else mbar_arrive_expect_tx(&full_bar[s], Cfg::kStageBytes);
+            if (PAIR) arrive_expect_cluster(bar, bytes);
+            else mbar_arrive_expect_tx(&full_bar[s], bytes);
           }
+          // First column of B in this CTA. (A box of a K-major B is as high as a whole share, so a narrow tile loads columns
+          // there that it does not use.)
+          const int b0 = t.n0 + static_cast<int>(rank) * (t.narrow ? Cfg::kLocalCols / 2 : Cfg::kLocalCols);
           auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, int z) {
             if constexpr (PAIR) tma_load_3d_pair(smem_u32(dst), map, bar, x, y, z);
             else tma_load_3d(dst, map, tail ? &tail_bar[s] : &full_bar[s], x, y, z);
@@ -475,9 +502,9 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
               const CUtensorMap* map = WEIGHTS ? &p.b[t.output] : &p.b[segment];
 #pragma unroll
               for (int c = 0; c < Cfg::kLocalCols / 64; ++c)
-                load(b + c * 8192, map, t.n0 + static_cast<int>(rank) * Cfg::kLocalCols + 64 * c, k0, z);
+                if (c == 0 || !t.narrow) load(b + c * 8192, map, b0 + 64 * c, k0, z);
             } else {
-              load(b, &p.b[segment], k0, t.n0 + static_cast<int>(rank) * Cfg::kLocalCols, z);
+              load(b, &p.b[segment], k0, b0, z);
             }
           }
         }
@@ -489,7 +516,8 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMAs
     if (leader && elect_one_sync()) {
-      constexpr uint32_t idesc = idesc_bf16(kTileM, Cfg::kBN, A_MN, B_MN);
+      constexpr uint32_t idesc_wide = idesc_bf16(kTileM, Cfg::kBN, A_MN, B_MN);
+      constexpr uint32_t idesc_narrow = idesc_bf16(kTileM, Cfg::kBN / 2, A_MN, B_MN);
       auto commit = [&](uint64_t* bar) {
         if constexpr (PAIR) {
           mma_commit_pair(smem_u32(bar));
@@ -504,6 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       int e = 0;
       for (long long unit = first_unit; unit < units && ok; unit += unit_step) {
         const Tile t = tile_at(unit, e);
+        const uint32_t idesc = t.narrow ? idesc_narrow : idesc_wide;
         for (int step = 0; step < t.steps; ++step, at.next()) {
           const bool first = PLANES > 1 || step == 0;
           const int buf = acc.stage;
@@ -577,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
     }
   } else if (warp >= kEpiWarp0) {
     // -------------------------------------------------------------- epilogue
-    if constexpr (PLANES > 1) regs_increase<Cfg::kRegsEpilogue>();
+    if constexpr (kSplit) regs_increase<Cfg::kRegsEpilogue>();
     constexpr int kCols = Cfg::kBN / 2;  // columns of a thread: half a row of the tile
     constexpr int kSpanCols = kSpan<Out>;
     const int quarter = warp % 4, half = (warp - kEpiWarp0) / 4;
@@ -598,15 +627,15 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       const int row0 = t.row0 + quarter * 32;
       const int rows = min(max(t.row_end - row0, 0), 32);
       const long long first = (WEIGHTS ? static_cast<long long>(t.expert) * p.m : 0) + row0;
-      // g and u of the SwiGLU backward travel a span ahead, the first one's while the MMAs run.
-      Span next_g, next_u;
-      const __nv_bfloat16* g_rows = static_cast<const __nv_bfloat16*>(p.in[0]) + first * p.ld_in;
-      const __nv_bfloat16* u_rows = static_cast<const __nv_bfloat16*>(p.in[1]) + first * p.ld_in;
+      // g and u of the SwiGLU backward travel 32 columns ahead, the first ones while the MMAs run.
+      Quarter next_g[4], next_u[4];
+      const float* g_rows = static_cast<const float*>(p.in[0]) + first * p.ld_in;
+      const float* u_rows = static_cast<const float*>(p.in[1]) + first * p.ld_in;
       if constexpr (EPI == kSwiGLUBwd) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          next_g.load_quarter(i, lane, g_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
-          next_u.load_quarter(i, lane, u_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
+          next_g[i].load(i, lane, g_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
+          next_u[i].load(i, lane, u_rows, p.ld_in, rows, t.n0 + half * kCols, p.n);
         }
       }
       float acc[PLANES > 1 ? kCols : 1];
@@ -691,8 +720,8 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
             columns(c + kCols / 2, up);
           }
           const int col = t.n0 + half * (kCols / 2) + c;
-          store_span<Out>(mine, lane, static_cast<Out*>(p.out[0]) + first * p.ld[0], p.ld[0], rows, col, p.n, gate);
-          store_span<Out>(mine, lane, static_cast<Out*>(p.out[1]) + first * p.ld[1], p.ld[1], rows, col, p.n, up);
+          store_kept(mine, lane, static_cast<float*>(p.out[0]) + first * p.ld[0], p.ld[0], rows, col, p.n, gate);
+          store_kept(mine, lane, static_cast<float*>(p.out[1]) + first * p.ld[1], p.ld[1], rows, col, p.n, up);
 #pragma unroll
           for (int i = 0; i < kSpanCols; ++i) up[i] *= gate[i] * sigmoid(gate[i]);
           store_operand<PLANES>(mine, lane, static_cast<__nv_bfloat16*>(p.out[2]) + first * p.ld[2], p.plane, p.ld[2], rows,
@@ -720,11 +749,11 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
             float d[8], g[8], u[8];
             OutTraits<float>::unpack(*reinterpret_cast<const uint4*>(mine + unit_at<8>(r, (lane % 4) * 2)), d);
             OutTraits<float>::unpack(*reinterpret_cast<const uint4*>(mine + unit_at<8>(r, (lane % 4) * 2 + 1)), d + 4);
-            OutTraits<__nv_bfloat16>::unpack(next_g.v[i], g);
-            OutTraits<__nv_bfloat16>::unpack(next_u.v[i], u);
+            next_g[i].get(g);
+            next_u[i].get(u);
             if (c + 32 < kCols) {
-              next_g.load_quarter(i, lane, g_rows, p.ld_in, rows, t.n0 + half * kCols + c + 32, p.n);
-              next_u.load_quarter(i, lane, u_rows, p.ld_in, rows, t.n0 + half * kCols + c + 32, p.n);
+              next_g[i].load(i, lane, g_rows, p.ld_in, rows, t.n0 + half * kCols + c + 32, p.n);
+              next_u[i].load(i, lane, u_rows, p.ld_in, rows, t.n0 + half * kCols + c + 32, p.n);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -769,6 +798,15 @@ cudaError_t launch_one(const Params& p, long long units, int sms, cudaStream_t s
   const auto kernel = ragged_kernel<PLANES, PAIR, WEIGHTS, B_MN, EPI>;
   static host::PerDeviceOnce once;
   cudaError_t err = cudaSuccess;
+  if (split_registers(PLANES, EPI)) {
+    // A split above the launch's registers would wait forever.
+    static const int registers = [&] {
+      cudaFuncAttributes a = {};
+      return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (registers * kThreads < static_cast<int>(128 * Cfg::kRegsControl + 256 * Cfg::kRegsEpilogue))
+      return cudaErrorInvalidConfiguration;
+  }
   once.run([&] { err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes); });
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};

@@ -20,6 +20,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const StageParams p, bool ve
     const long long row = i / per_row;  // of all batches
     const long long c0 = (i - row * per_row) * 8;
     const long long b = row / p.rows, r = row - b * p.rows;
+    if (p.offsets != nullptr && p.offsets[b + 1] <= (b == 0 ? 0 : p.offsets[b])) continue;
     const long long at = b * p.stride_batch + r * p.stride_row + c0 * p.stride_col;
     uint4 words[3];
     if (p.src_bf16) {
