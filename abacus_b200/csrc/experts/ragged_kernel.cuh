@@ -16,7 +16,7 @@
 // registers rounding to nearest, so the error is that of an fp32 sum.
 //
 // Roles of a CTA (384 threads): warp 0 loads tiles by TMA, warp 1 issues the
-// MMAs, warp 2 clears the rows of a tile that belong to the next expert (the
+// MMAs, warps 2 and 3 clear the rows of a tile that belong to the next expert (the
 // contraction of `weights` runs over rows, so they would be added; both
 // operands are cleared, so that nothing infinite meets a zero), warps 4-11 are
 // the epilogue. In a pair (cta_group::2) each CTA holds 128 of the tile's 256
@@ -102,10 +102,6 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* map, 
 __device__ __forceinline__ void arrive_expect_cluster(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
-}
-
-__device__ __forceinline__ void arrive_release_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Bounded wait. The common header's wait reads the nanosecond timer as soon as a barrier is not ready, which takes about
@@ -576,30 +572,34 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       }
       drain<kStages>(empty_bar, at);
     }
-  } else if (warp == 2) {
+  } else if (warp < kEpiWarp0) {
     // -------------------------------------------------------------- rows of the next expert
+    // Both warps take every turn (a wait that ran out only stops their work), since they meet at a barrier in each.
     if constexpr (WEIGHTS) {
-      long long it = 0;
+      Position<kStages> at;
       uint32_t parity = 0;  // of each stage's tail barrier
+      bool ok = true;
       int e = 0;
       for (long long unit = first_unit; unit < units; unit += unit_step) {
         const Tile t = tile_at(unit, e);
-        it += t.steps;
         const int valid = t.k_rows % kDepth;
+        const int s = (at.stage + t.steps - 1) % kStages;  // of the tile's last step
+        at.stage = (at.stage + t.steps) % kStages;
         if (valid == 0) continue;  // no rows at all, or whole stages
-        const int s = static_cast<int>((it - 1) % kStages);
-        if (!wait_bar_warp(&tail_bar[s], (parity >> s) & 1, p.status, kStatusTimeoutConvert)) break;
+        ok = ok && wait_bar_warp(&tail_bar[s], (parity >> s) & 1, p.status, kStatusTimeoutConvert);
         parity ^= 1u << s;
-        // All chunks of a stage are 64 rows of 128 bytes; swizzling stays inside a row.
-        uint8_t* stage = smem + s * Cfg::kStageBytes;
-        const int units16 = (kDepth - valid) * 8;
-        for (int chunk = 0; chunk < Cfg::kStageBytes / 8192; ++chunk)
-          for (int u = lane; u < units16; u += 32)
-            *reinterpret_cast<uint4*>(stage + chunk * 8192 + valid * 128 + u * 16) = make_uint4(0, 0, 0, 0);
+        if (ok) {
+          // All chunks of a stage are 64 rows of 128 bytes; swizzling stays inside a row.
+          uint8_t* stage = smem + s * Cfg::kStageBytes;
+          const int units16 = (kDepth - valid) * 8;
+          for (int chunk = warp - 2; chunk < Cfg::kStageBytes / 8192; chunk += 2)
+            for (int u = lane; u < units16; u += 32)
+              *reinterpret_cast<uint4*>(stage + chunk * 8192 + valid * 128 + u * 16) = make_uint4(0, 0, 0, 0);
+        }
         fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          if (PAIR) arrive_release_cluster(leader_addr(&full_bar[s]));
+        named_barrier_sync(2, 64);
+        if (ok && warp == 2 && lane == 0) {
+          if (PAIR) mbar_arrive_cluster(leader_addr(&full_bar[s]));
           else mbar_arrive(&full_bar[s]);
         }
       }

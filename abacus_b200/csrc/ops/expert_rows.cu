@@ -188,6 +188,8 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const T* __restrict__ x, 
   zero_tail<T, N>(xs, count, end, packs, warp, warps, lane);
 }
 
+constexpr int units_at_once(int n) { return n >= 8 ? 1 : n == 4 ? 2 : 4; }
+
 // out[t] = sum_k w(t, k) ys[slot(t, k)], or without weights the plain sum. A lane sums several units at once where they
 // are narrow, so that about as many bytes are in flight (at 8-byte units one at a time left half of the bandwidth unused;
 // two 16-byte bf16 units at a time cost registers and were slower, 63 us against 55 for 65536 tokens of 768).
@@ -195,7 +197,7 @@ template <class T, int N>
 __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ ys, const float* __restrict__ weights,
                                                       const int* __restrict__ slot, T* __restrict__ out, long long tokens,
                                                       int choices, long long packs) {
-  constexpr int kUnits = N >= 8 ? 1 : N == 4 ? 2 : 4;
+  constexpr int kUnits = units_at_once(N);
   const int lane = threadIdx.x % 32;
   const long long warp = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
   const long long warps = static_cast<long long>(gridDim.x) * blockDim.x / 32;
@@ -236,14 +238,15 @@ __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ ys, 
 }
 
 // GROUP choices of a token at a time, so that d out[t] is read once for them: two where the number of choices is even
-// (90 us against 95 one at a time for 65536 tokens, 2 choices, 768 bf16), one where it is odd (40 us against 51 two at a
-// time for 9001 tokens, 3 choices, 770 fp32).
+// (77 us for 65536 tokens, 2 choices, 768 bf16; 95 one at a time), one where it is odd (33 us for 9001 tokens, 3 choices,
+// 770 fp32; 51 two at a time).
 template <class T, int N, int GROUP>
 __global__ void __launch_bounds__(256) combine_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ ys,
                                                           const float* __restrict__ weights, const int* __restrict__ slot,
                                                           const int* __restrict__ end, T* __restrict__ dys,
                                                           float* __restrict__ dweights, long long tokens, int choices,
                                                           long long packs) {
+  constexpr int kUnits = units_at_once(N);
   const int lane = threadIdx.x % 32;
   const long long warp = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
   const long long warps = static_cast<long long>(gridDim.x) * blockDim.x / 32;
@@ -251,33 +254,45 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const T* __restrict__ 
   for (long long t = warp; t < tokens; t += warps) {
     const Pack<T, N>* d = reinterpret_cast<const Pack<T, N>*>(dout) + t * packs;
     for (int k = 0; k < choices; k += GROUP) {
-      long long s[GROUP];
+      // A dropped choice reads row 0 (loads without conditions overlap better) and stores nothing.
+      long long row[GROUP];
+      bool kept[GROUP], any = false;
       float w[GROUP], dot[GROUP];
 #pragma unroll
       for (int i = 0; i < GROUP; ++i) {
         const long long r = slot[t * choices + k + i];
-        s[i] = r < count ? r : -1;
+        kept[i] = r >= 0 && r < count;
+        any = any || kept[i];
+        row[i] = (kept[i] ? r : 0) * packs;
         w[i] = weights[t * choices + k + i];
         dot[i] = 0.f;
       }
+      if (any) {
 #pragma unroll 2
-      for (long long c = lane; c < packs; c += 32) {
-        const Pack<T, N> a = d[c];
-        Pack<T, N> y[GROUP];
+        for (long long c = lane; c < packs; c += 32 * kUnits) {
+          Pack<T, N> a[kUnits], y[GROUP][kUnits];
 #pragma unroll
-        for (int i = 0; i < GROUP; ++i)
-          if (s[i] >= 0) y[i] = reinterpret_cast<const Pack<T, N>*>(ys)[s[i] * packs + c];
+          for (int j = 0; j < kUnits; ++j) {
+            if (c + 32 * j >= packs) continue;
+            a[j] = d[c + 32 * j];
 #pragma unroll
-        for (int i = 0; i < GROUP; ++i) {
-          if (s[i] < 0) continue;
-          Pack<T, N> o;
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float g = to_float(a.v[e]);
-            dot[i] = fmaf(g, to_float(y[i].v[e]), dot[i]);
-            o.v[e] = from_float<T>(w[i] * g);
+            for (int i = 0; i < GROUP; ++i) y[i][j] = reinterpret_cast<const Pack<T, N>*>(ys)[row[i] + c + 32 * j];
           }
-          reinterpret_cast<Pack<T, N>*>(dys)[s[i] * packs + c] = o;
+#pragma unroll
+          for (int j = 0; j < kUnits; ++j) {
+            if (c + 32 * j >= packs) continue;
+#pragma unroll
+            for (int i = 0; i < GROUP; ++i) {
+              Pack<T, N> o;
+#pragma unroll
+              for (int e = 0; e < N; ++e) {
+                const float g = to_float(a[j].v[e]);
+                dot[i] = fmaf(g, to_float(y[i][j].v[e]), dot[i]);
+                o.v[e] = from_float<T>(w[i] * g);
+              }
+              if (kept[i]) reinterpret_cast<Pack<T, N>*>(dys)[row[i] + c + 32 * j] = o;
+            }
+          }
         }
       }
 #pragma unroll
@@ -287,7 +302,7 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const T* __restrict__ 
       }
       if (lane == 0) {
 #pragma unroll
-        for (int i = 0; i < GROUP; ++i) dweights[t * choices + k + i] = dot[i];
+        for (int i = 0; i < GROUP; ++i) dweights[t * choices + k + i] = kept[i] ? dot[i] : 0.f;
       }
     }
   }
@@ -414,6 +429,10 @@ void expert_combine(torch::Tensor ys, c10::optional<torch::Tensor> weights, torc
                     weights->numel() == tokens * choices,
                 "weights must be a contiguous fp32 CUDA tensor of the slots' shape");
   if (tokens == 0 || dim == 0) return;
+  if (choices == 0) {
+    out.zero_();
+    return;
+  }
   const int element = static_cast<int>(ys.element_size());
   with_pack(ys, pack_of(dim, dim, element, {ys.data_ptr(), out.data_ptr()}), [&](auto zero, auto n) {
     using T = decltype(zero);
