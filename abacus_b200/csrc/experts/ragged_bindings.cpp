@@ -80,7 +80,8 @@ void check_kept(const torch::Tensor& t, const torch::Tensor& like, int64_t rows,
 void check_written(const torch::Tensor& t, const torch::Tensor& like, int64_t planes, int64_t rows, int64_t cols, const char* name) {
   check_operand(t, 3, name);
   TORCH_CHECK(t.device() == like.device() && t.size(0) == planes && t.size(1) == rows && t.size(2) == cols &&
-                  t.stride(1) % 8 == 0 && t.stride(1) >= (cols + 7) / 8 * 8 && t.stride(0) == rows * t.stride(1),
+                  t.stride(1) % 8 == 0 && t.stride(1) >= (cols + 7) / 8 * 8 &&
+                  (rows == 0 || t.stride(0) == rows * t.stride(1)),
               name, " must be (planes, rows, columns) with padded rows");
 }
 

@@ -212,8 +212,16 @@ struct Rows32 {
     } else {
       const int unit = lane / Traits::kPerUnit, in = lane % Traits::kPerUnit;
       if (col0 + lane < cols) {
-        for (int r = 0; r < rows; ++r)
-          base[r * ld + col0 + lane] = reinterpret_cast<const Out*>(staging + unit_at<kUnits>(r, unit))[in];
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+          Out v8[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            v8[i] = reinterpret_cast<const Out*>(staging + unit_at<kUnits>(r0 + i, unit))[in];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (r0 + i < rows) base[(r0 + i) * ld + col0 + lane] = v8[i];
+        }
       }
     }
   }

@@ -1,4 +1,4 @@
-// AdamW with 8-bit moments (see adamw8.cu).
+// AdamW with 8-bit moments (see adamw8.cpp).
 #pragma once
 #include <torch/extension.h>
 #include <vector>

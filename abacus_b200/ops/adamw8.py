@@ -15,7 +15,7 @@ same inputs give the same outputs, on the CPU as on the GPU. A second moment
 that is not zero never rounds to zero. A gradient that is infinite or NaN
 spoils its own element (moments NaN, as in 32 bits), not its block.
 
-CUDA tensors run on ``csrc/ops/adamw8.cu`` (one launch for up to 128 tensors);
+CUDA tensors run on ``csrc/ops/adamw8_kernel.cu`` (one launch for up to 128 tensors);
 CPU tensors run the formulation below.
 """
 from __future__ import annotations

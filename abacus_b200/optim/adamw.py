@@ -25,7 +25,7 @@ Execution: parameters are grouped by (device, step count). On CUDA each group
 is one multi-tensor kernel launch per 36 tensors (``csrc/ops/embed_ce_adamw.cu``);
 elsewhere each group runs the same update as ``torch._foreach_*`` operations,
 which apply the formulas above element by element in the order written. 8-bit
-groups are one launch per 128 tensors (``csrc/ops/adamw8.cu``).
+groups are one launch per 128 tensors (``csrc/ops/adamw8_kernel.cu``).
 """
 from __future__ import annotations
 

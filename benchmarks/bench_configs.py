@@ -54,6 +54,9 @@ def parse_args():
     p.add_argument("--precision", choices=("fp32", "tf32"), default="fp32")
     p.add_argument("--global-batch", type=int, default=None)
     p.add_argument("--seq-len", type=int, default=None)
+    p.add_argument("--ragged", action="store_true", help="moe, one GPU: the dropless operators in place of capacity slabs")
+    p.add_argument("--expert-dtype", choices=("fp32", "bf16"), default="fp32", help="moe with --ragged: type of the experts' products")
+    p.add_argument("--state-bits", type=int, choices=(8, 32), default=32, help="moe: AdamW's moments")
     p.add_argument("--layers", type=int, default=None, help="override the layer count (smoke runs only)")
     return p.parse_args()
 
@@ -84,13 +87,14 @@ def build_abacus(cfg, args, world, device):
         if world > 1:
             mesh.init_mesh(dp=world, ep=world)
         model = TransformerMoe(768, 12, 64, args.layers or 12, VOCAB, 8, 2, hidden_dim=1536, router="softmax",
-                               capacity_factor=1.25, expert_parallel=world > 1, expert_data_parallel=world > 1)
+                               capacity_factor=1.25, expert_parallel=world > 1, expert_data_parallel=world > 1,
+                               ragged=args.ragged, expert_dtype=torch.bfloat16 if args.expert_dtype == "bf16" else None)
         parallel = None
         if world > 1:
             model = model.to(device)
             expert_params = [p for n, p in model.named_parameters() if ".moe.w_" in n]
             parallel = DataParallel(model, exclude=expert_params, token_weighted=False)
-        return Trainer(model, parallel, total_steps=1000, device=device), "ep%d+dp%d" % (world, world), False
+        return Trainer(model, parallel, total_steps=1000, device=device, state_bits=args.state_bits), "ep%d+dp%d" % (world, world), False
     # cppp
     from abacus_b200.parallel.pipeline_parallel import PipelineParallel
     from abacus_b200.transformer import PipelineStage

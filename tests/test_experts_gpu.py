@@ -223,6 +223,42 @@ def test_bad_offsets_stay_in_bounds():
         check_status()
 
 
+def test_no_rows():
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.zeros(0, 24, device="cuda", dtype=dtype, requires_grad=True)
+        mats = [torch.randn(3, *s, device="cuda").to(dtype).requires_grad_() for s in ((24, 40), (24, 40), (40, 24))]
+        off = _offsets([0, 0, 0])
+        for y, args in ((experts.ragged_matmul(x, mats[0], off), (x, mats[0])), (experts.ragged_swiglu_mlp(x, *mats, off), (x, *mats))):
+            assert y.shape[0] == 0
+            for grad, t in zip(torch.autograd.grad(y, args, torch.zeros_like(y)), args):
+                assert grad.shape == t.shape and torch.all(grad == 0)
+
+
+def test_differentiable_once():
+    off = _offsets([4, 3])
+    x = torch.randn(7, 16, device="cuda", requires_grad=True)
+    w = torch.randn(2, 16, 16, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        torch.autograd.grad(experts.ragged_matmul(x, w, off).sum(), x, create_graph=True)
+    plan = experts.expert_plan(torch.zeros(7, 1, dtype=torch.int64, device="cuda"), 2)
+    with pytest.raises(RuntimeError, match="not differentiable twice"):
+        torch.autograd.grad(experts.dispatch_tokens(x, plan).sum(), x, create_graph=True)
+
+
+def test_only_the_gradients_that_are_asked_for():
+    off = _offsets([5, 9])
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.randn(14, 32, device="cuda").to(dtype)
+        mats = [torch.randn(2, *s, device="cuda").to(dtype) for s in ((32, 48), (32, 48), (48, 32))]
+        full = [t.clone().requires_grad_() for t in (x, *mats)]
+        want = torch.autograd.grad(experts.ragged_swiglu_mlp(*full, off).float().square().sum(), full)
+        for i in range(4):
+            args = [x, *mats]
+            args[i] = args[i].clone().requires_grad_()
+            (got,) = torch.autograd.grad(experts.ragged_swiglu_mlp(*args, off).float().square().sum(), args[i])
+            assert torch.equal(got, want[i])
+
+
 def test_refusals():
     x = torch.zeros(4, 8, device="cuda")
     w = torch.zeros(300, 8, 8, device="cuda")
