@@ -51,13 +51,24 @@ __device__ __forceinline__ float largest(float top, float x) {
 // Over the warp, as bits (of numbers that are not negative, which order as their bits do, NaN last).
 __device__ __forceinline__ unsigned warp_top(float top) { return __reduce_max_sync(0xffffffffu, __float_as_uint(top)); }
 
-// The special-function unit's root (within 2^-22): a last-bit error of u is far below its rounding to 8 bits, and
-// the correctly rounded root is a dozen instructions in a kernel that is short of issue slots.
+// The special-function unit's root and 1 / (2 root); tiny enough not to matter, the sum keeps the latter finite at zero.
 __device__ __forceinline__ float root(float x) {
   float y;
   asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float half_over_root(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(x, 4.f, 0x1p-126f)));
+  return y;
+}
+
+// The root of x rounded to nearest, from an approximation s of it: one step of Heron's method, s + (x - s^2) / (2 s) with
+// the difference exact, is off by the square of s's error, so its rounding is the root's but for one number in a million.
+// The moment that is kept needs that (which of two codes a number gets depends on its last bit where it meets its
+// threshold, and one code is an eighth of it), the weight's update does not. The correctly rounded library root does the
+// same and made the kernel 11 to 100 % slower with the registers it takes.
+__device__ __forceinline__ float polished(float s, float x) { return fmaf(fmaf(-s, s, x), half_over_root(x), s); }
 
 // The e4m3 code of x, rounded stochastically by 16 random bits; |x| < 256. Times 2^-120, e4m3's smallest normal number
 // (2^-6) is fp32's (2^-126) and the two formats' exponent fields agree, subnormal numbers included: the code is the upper
@@ -144,8 +155,9 @@ __global__ void __launch_bounds__(kAdam8Warps * 32, 6) adamw8_kernel(const __gri
       const float gi = g[h][e];
       const float mi = __fadd_rn(__fmul_rn(m[h][e] * ms, s.b1), __fmul_rn(gi, s.c1));
       const float uo = u[h][e] * us;
-      const float ui = root(__fadd_rn(__fmul_rn(__fmul_rn(uo, uo), s.b2), __fmul_rn(__fmul_rn(gi, gi), s.c2)));
-      w[h][e] = w[h][e] * s.decay - __fdividef(mi * s.step_size, ui + s.eps);
+      const float vi = __fadd_rn(__fmul_rn(__fmul_rn(uo, uo), s.b2), __fmul_rn(__fmul_rn(gi, gi), s.c2));
+      const float near = root(vi), ui = polished(near, vi);
+      w[h][e] = w[h][e] * s.decay - __fdividef(mi * s.step_size, near + s.eps);
       m[h][e] = mi;
       u[h][e] = ui;
       m_max = largest(m_max, mi);

@@ -96,3 +96,24 @@ def test_refusals():
         adamw8.step_(*gpu[:3], [gpu[3][0][:1]], *gpu[4:], lr=1e-3, step=1)
     with pytest.raises(RuntimeError, match="one CUDA device"):
         adamw8.step_(gpu[0], [gpu[1][0].cpu()], *gpu[2:], lr=1e-3, step=1)
+
+
+def test_codes_are_the_cpu_formulation_s_over_many_elements():
+    """Both sides compute the moments with the same roundings (the kernel's root is rounded to nearest but for one number
+    in a million, which then changes a code with a chance below 2^-16), so a million elements give the same codes, step
+    after step, and weights stay together although an unlike code would change an update by an eighth."""
+    n = 1 << 20
+    g = torch.Generator().manual_seed(11)
+    # Magnitudes over twenty octaves, neighbours far apart, zeros among them.
+    grad = torch.randn(n, generator=g) * torch.exp2(torch.randint(-20, 0, (n,), generator=g).float()) * (torch.rand(n, generator=g) > 0.1)
+    tensors = [(torch.randn(n, generator=g), grad, adamw8.fresh_state(n, "cpu"))]
+    gpu, cpu = _lists(tensors, "cuda"), _lists(tensors, "cpu")
+    for step in range(1, 6):
+        scale = 0.5 + torch.rand(n, generator=g)
+        cpu[1][0].copy_(grad * scale)
+        gpu[1][0].copy_(cpu[1][0])
+        adamw8.step_(*gpu, lr=1e-3, step=step)
+        adamw8.step_(*cpu, lr=1e-3, step=step)
+        for which in (2, 4):
+            assert (gpu[which][0].cpu().float() != cpu[which][0].float()).sum() <= 1
+    torch.testing.assert_close(gpu[0][0].cpu(), cpu[0][0], rtol=1e-6, atol=1e-5)
