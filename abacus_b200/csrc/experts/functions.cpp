@@ -5,8 +5,14 @@
 // None of them is differentiable twice; a backward pass that records a graph is refused.
 #include <torch/extension.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include "../common/host.h"
 #include "../ops/expert_rows.h"
 #include "bindings.h"
+#include "few.h"
+#include "ragged.h"
 
 namespace abacus {
 namespace experts {
@@ -73,16 +79,81 @@ struct Combine : torch::autograd::Function<Combine> {
   }
 };
 
+// Whether TMA can read `t` where it lies.
+bool read_in_place(const Tensor& t) {
+  const int64_t d = t.dim();
+  if (t.scalar_type() != torch::kBFloat16 || t.stride(d - 1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0)
+    return false;
+  bool aligned = t.size(d - 2) <= 1 || t.stride(d - 2) >= t.size(d - 1);
+  for (int64_t i = 0; i < d - 1; ++i) aligned = aligned && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) > 0));
+  return aligned;
+}
+
 // `t` as the product kernels read it: bf16 planes first, rows 16-byte aligned. bf16 tensors laid out so already are used in
 // place. With offsets, `t` holds the experts' matrices, and those of experts without rows are left out of a copy.
 Tensor operand(const Tensor& t, int64_t planes, c10::optional<Tensor> offsets = c10::nullopt) {
-  const int64_t d = t.dim();
-  if (t.scalar_type() == torch::kBFloat16 && t.stride(d - 1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) {
-    bool aligned = t.size(d - 2) <= 1 || t.stride(d - 2) >= t.size(d - 1);
-    for (int64_t i = 0; i < d - 1; ++i) aligned = aligned && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) > 0));
-    if (aligned) return t.unsqueeze(0);
+  return read_in_place(t) ? t.unsqueeze(0) : ragged::stage(t, planes, offsets);
+}
+
+// ---------------------------------------------------------------- few rows (few.cu)
+// Few rows, and matrices that the tensor-core path would copy first: fp32 ones, and bf16 ones whose rows are not whole
+// 16-byte units. Other bf16 matrices are read in place there, and it is as fast or faster from one row an expert on
+// (32 experts of 2048 x 2048: 50 us against 61 with one row each). The choice goes by sizes and type alone, so that a
+// tensor's layout does not change its product's bits.
+bool few(const Tensor& x, const Tensor& w, const Tensor& offsets) {
+  const bool bf16 = w.scalar_type() == torch::kBFloat16;
+  return ragged::few_rows(x.size(0), offsets.numel() - 1, bf16) && (!bf16 || w.size(2) % 8 != 0);
+}
+
+// Matrices whose rows lie in one piece.
+Tensor rows_in_one_piece(const Tensor& w) { return w.stride(2) == 1 ? w : w.contiguous(); }
+
+ragged::FewParams few_params(const Tensor& a, const Tensor& b, const Tensor& offsets, const Tensor& out) {
+  ragged::FewParams p = {};
+  p.a = a.data_ptr();
+  p.b = b.data_ptr();
+  p.out = out.data_ptr();
+  p.a_bf16 = a.scalar_type() == torch::kBFloat16;
+  p.b_bf16 = b.scalar_type() == torch::kBFloat16;
+  p.out_bf16 = out.scalar_type() == torch::kBFloat16;
+  p.ld_a = a.stride(0);
+  p.offsets = offsets.data_ptr<int>();
+  p.experts = static_cast<int>(offsets.numel() - 1);
+  p.rows = static_cast<int>(a.size(0));
+  return p;
+}
+
+void launched(cudaError_t err) {
+  C10_CUDA_CHECK(err);
+  host::note_launch();
+}
+
+// out = a times the experts' matrices, or their transposes (with `add` added).
+void few_rows_product(const Tensor& a, const Tensor& w, const Tensor& offsets, const Tensor& out, bool transposed,
+                      const Tensor& add = Tensor()) {
+  if (a.size(0) == 0) return;
+  const c10::cuda::CUDAGuard guard(a.device());
+  auto p = few_params(a, w, offsets, out);
+  p.ld_b = w.stride(1);
+  p.stride_b = w.stride(0);
+  p.ld_out = out.stride(0);
+  p.k = static_cast<int>(w.size(transposed ? 2 : 1));
+  p.n = static_cast<int>(w.size(transposed ? 1 : 2));
+  if (add.defined()) {
+    p.add = add.data_ptr<float>();
+    p.ld_add = add.stride(0);
   }
-  return ragged::stage(t, planes, offsets);
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  launched(transposed ? launch_few_transposed(p, stream) : launch_few(p, stream));
+}
+
+void few_weights(const Tensor& a, const Tensor& b, const Tensor& offsets, const Tensor& out) {
+  const c10::cuda::CUDAGuard guard(a.device());
+  auto p = few_params(a, b, offsets, out);
+  p.ld_b = b.stride(0);
+  p.m = static_cast<int>(out.size(1));
+  p.n = static_cast<int>(out.size(2));
+  launched(launch_few_weights(p, at::cuda::getCurrentCUDAStream()));
 }
 
 Tensor like_matrix(const Tensor& w) { return torch::empty(w.sizes(), w.options()); }
@@ -96,6 +167,14 @@ Tensor padded(int64_t planes, int64_t rows, int64_t cols, torch::TensorOptions o
 
 struct RaggedMatmul : torch::autograd::Function<RaggedMatmul> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t planes) {
+    if (few(x, w, offsets)) {
+      const auto xr = walkable(x), wr = rows_in_one_piece(w);
+      ctx->save_for_backward({xr, wr, offsets});
+      ctx->saved_data["planes"] = static_cast<int64_t>(0);
+      auto y = torch::empty({x.size(0), w.size(2)}, x.options());
+      few_rows_product(xr, wr, offsets, y, false);
+      return y;
+    }
     // The backward reads x as an operand: where that is a copy it is kept in place of x (6 bytes an element in fp32; w's,
     // which would stay for the whole forward of a model, is made again).
     const auto xo = operand(x, planes);
@@ -110,8 +189,20 @@ struct RaggedMatmul : torch::autograd::Function<RaggedMatmul> {
     const auto saved = ctx->get_saved_variables();
     const auto &x = saved[0], &w = saved[1], &offsets = saved[2];
     const int64_t planes = ctx->saved_data["planes"].toInt();
-    const auto dy = operand(grads[0], planes);
     Tensor dx, dw;
+    if (planes == 0) {
+      const auto dy = walkable(grads[0]);
+      if (ctx->needs_input_grad(0)) {
+        dx = torch::empty(x.sizes(), w.options());
+        few_rows_product(dy, w, offsets, dx, true);
+      }
+      if (ctx->needs_input_grad(1)) {
+        dw = like_matrix(w);
+        few_weights(x, dy, offsets, dw);
+      }
+      return {dx, dw, Tensor(), Tensor()};
+    }
+    const auto dy = operand(grads[0], planes);
     if (ctx->needs_input_grad(0)) {
       dx = torch::empty({x.size(1), x.size(2)}, w.options());
       ragged::rows({dy}, {operand(w, planes, offsets)}, offsets, dx, true);
@@ -127,10 +218,55 @@ struct RaggedMatmul : torch::autograd::Function<RaggedMatmul> {
 // The kernels write h and the gradients of gate and up as the operands (bf16 planes) of the products that read them; the
 // operands of x and h are kept for the backward in place of the tensors.
 struct RaggedSwiGLU : torch::autograd::Function<RaggedSwiGLU> {
+  static variable_list backward_of_few(AutogradContext* ctx, const variable_list& saved, const Tensor& grad) {
+    const auto &x = saved[0], &w_gate = saved[1], &w_up = saved[2], &w_down = saved[3], &offsets = saved[4], &g = saved[5],
+               &u = saved[6], &h = saved[7];
+    const auto dy = walkable(grad);
+    const auto dgu = torch::empty({2, g.size(0), g.size(1)}, g.options());
+    const auto dg = dgu[0], du = dgu[1];
+    few_rows_product(dy, w_down, offsets, dg, true);  // dh, in the place of dg
+    if (g.numel() > 0) {
+      const c10::cuda::CUDAGuard guard(x.device());
+      launched(ragged::launch_few_swiglu_bwd(dg.data_ptr<float>(), g.data_ptr<float>(), u.data_ptr<float>(),
+                                             dg.data_ptr<float>(), du.data_ptr<float>(), g.numel(),
+                                             at::cuda::getCurrentCUDAStream()));
+    }
+    variable_list out(6);
+    if (ctx->needs_input_grad(0)) {
+      const auto part = torch::empty(x.sizes(), g.options());
+      out[0] = torch::empty(x.sizes(), w_gate.options());
+      few_rows_product(dg, w_gate, offsets, part, true);
+      few_rows_product(du, w_up, offsets, out[0], true, part);
+    }
+    const Tensor* matrices[3] = {&w_gate, &w_up, &w_down};
+    for (int i = 0; i < 3; ++i) {
+      if (!ctx->needs_input_grad(i + 1)) continue;
+      out[i + 1] = like_matrix(*matrices[i]);
+      few_weights(i < 2 ? x : h, i == 0 ? dg : i == 1 ? du : dy, offsets, out[i + 1]);
+    }
+    return out;
+  }
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
                         const Tensor& w_down, const Tensor& offsets, int64_t planes) {
     const int64_t rows = x.size(0), hidden = w_gate.size(2);
     const auto kept = x.options().dtype(torch::kFloat32);
+    if (few(x, w_gate, offsets) || few(x, w_down, offsets)) {
+      // gate, up and h stay fp32 throughout.
+      const auto xr = walkable(x), wg = rows_in_one_piece(w_gate), wu = rows_in_one_piece(w_up), wd = rows_in_one_piece(w_down);
+      const auto guh = torch::empty({3, rows, hidden}, kept);
+      const auto g = guh[0], u = guh[1], h = guh[2];
+      auto y = torch::empty({rows, w_down.size(2)}, x.options());
+      few_rows_product(xr, wg, offsets, g, false);
+      few_rows_product(xr, wu, offsets, u, false);
+      if (rows > 0) {
+        const c10::cuda::CUDAGuard guard(x.device());
+        launched(ragged::launch_few_swiglu(g.data_ptr<float>(), u.data_ptr<float>(), h.data_ptr<float>(), g.numel(),
+                                           at::cuda::getCurrentCUDAStream()));
+      }
+      few_rows_product(h, wd, offsets, y, false);
+      ctx->save_for_backward({xr, wg, wu, wd, offsets, g, u, h});
+      return y;
+    }
     const auto g = padded(0, rows, hidden, kept), u = padded(0, rows, hidden, kept);
     const auto h = padded(planes, rows, hidden, x.options().dtype(torch::kBFloat16));
     auto y = torch::empty({rows, w_down.size(2)}, x.options());
@@ -145,6 +281,7 @@ struct RaggedSwiGLU : torch::autograd::Function<RaggedSwiGLU> {
     const auto saved = ctx->get_saved_variables();
     const auto &x = saved[0], &w_gate = saved[1], &w_up = saved[2], &w_down = saved[3], &offsets = saved[4], &g = saved[5],
                &u = saved[6], &h = saved[7];
+    if (h.dim() == 2) return backward_of_few(ctx, saved, grads[0]);
     const int64_t planes = h.size(0), rows = g.size(0), hidden = g.size(1);
     const auto dy = operand(grads[0], planes);
     const auto dg = padded(planes, rows, hidden, h.options()), du = padded(planes, rows, hidden, h.options());
@@ -184,6 +321,8 @@ void check_products(const Tensor& x, const Tensor& w, const char* name, int64_t 
 void check_offsets(const Tensor& offsets) {
   TORCH_CHECK_VALUE(offsets.dim() == 1 && offsets.numel() >= 2 && offsets.scalar_type() == torch::kInt32,
                     "offsets must be int32 of shape (experts + 1,), got ", offsets.sizes(), " ", offsets.scalar_type());
+  TORCH_CHECK(offsets.numel() - 1 <= ragged::kMaxExperts, "ragged products take at most ", ragged::kMaxExperts,
+              " experts, got ", offsets.numel() - 1);
 }
 
 }  // namespace

@@ -116,6 +116,62 @@ def test_swiglu_mlp_and_gradients(kind, tol, counts, d, hidden):
         assert _off(a, b) <= tol
 
 
+FEW = {
+    "a row": ([1], 0),
+    "a row of many experts, rows of nobody": ([0] * 20 + [1] + [0] * 5, 30),
+    "each number of rows of a block": ([1, 2, 3, 4, 5, 8, 9, 16, 17] + [0] * 9, 2),
+    "most in one expert": ([0, 3, 120, 0, 0, 0, 0, 0, 1] + [0] * 24, 0),
+    "nobody": ([0, 0, 0], 5),
+}
+
+
+@pytest.mark.parametrize("kind,tol", [("bf16", BF16), ("fp32", 2e-6)])
+@pytest.mark.parametrize("counts,idle", FEW.values(), ids=FEW.keys())
+@pytest.mark.parametrize("d,n", [(1, 1), (8, 16), (7, 13), (72, 1100), (1033, 35), (520, 2056)])
+def test_products_of_few_rows(kind, tol, counts, idle, d, n):
+    """fp32 sums of up to 2056 products added in short runs: a few 2^-24 of the norm."""
+    dtype = torch.bfloat16 if kind == "bf16" else torch.float32
+    rows = sum(counts) + idle
+    assert rows <= 4 * len(counts) and rows <= 256  # what takes the kernels for few rows (fp32, and bf16 of odd widths)
+    g = torch.Generator(device="cuda").manual_seed(d + n)
+    x = torch.randn(rows, d, device="cuda", generator=g).to(dtype)
+    w = torch.randn(len(counts), d, n, device="cuda", generator=g).to(dtype)
+    dy = torch.randn(rows, n, device="cuda", generator=g).to(dtype)
+    want = _exact_products(x, w, dy, counts)
+    x[sum(counts):] = float("nan")
+    dy[sum(counts):] = float("inf")
+    got = _run(x, w, dy, _offsets(counts))
+    for a, b in zip(got, want):
+        assert a.dtype == dtype and torch.isfinite(a).all() and _off(a, b) <= tol
+    # Layouts: a slice of wider rows, matrices seen through a transpose.
+    wide = torch.zeros(rows, d + 3, device="cuda", dtype=dtype)
+    wide[:, 1 : d + 1] = x
+    for a, b in zip(_run(wide[:, 1 : d + 1], w.transpose(1, 2).contiguous().transpose(1, 2), dy, _offsets(counts)), got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind,tol", [("bf16", 3 * BF16), ("fp32", 8e-6)])
+@pytest.mark.parametrize("counts,idle", FEW.values(), ids=FEW.keys())
+@pytest.mark.parametrize("d,hidden", [(7, 13), (136, 264)])
+def test_swiglu_mlp_of_few_rows(kind, tol, counts, idle, d, hidden):
+    dtype = torch.bfloat16 if kind == "bf16" else torch.float32
+    rows, e = sum(counts) + idle, len(counts)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    x = torch.randn(rows, d, device="cuda", generator=g).to(dtype)
+    mats = [(torch.randn(e, *s, device="cuda", generator=g) * s[0] ** -0.5).to(dtype) for s in ((d, hidden), (d, hidden), (hidden, d))]
+    dy = torch.randn(rows, d, device="cuda", generator=g).to(dtype)
+    xd, md = x.double().requires_grad_(), [m.double().requires_grad_() for m in mats]
+    parts = [(torch.nn.functional.silu(xd[a:b] @ md[0][i]) * (xd[a:b] @ md[1][i])) @ md[2][i] for i, (a, b) in _spans(counts)]
+    want_y = torch.cat([*parts, xd.new_zeros(idle, d)])
+    want = [want_y, *torch.autograd.grad(want_y, (xd, *md), dy.double())]
+    x[sum(counts):] = float("inf")
+    dy[sum(counts):] = float("nan")
+    x, mats = x.requires_grad_(), [m.requires_grad_() for m in mats]
+    y = experts.ragged_swiglu_mlp(x, *mats, _offsets(counts))
+    for a, b in zip([y, *torch.autograd.grad(y, (x, *mats), dy)], want):
+        assert a.dtype == dtype and torch.isfinite(a).all() and _off(a, b) <= tol
+
+
 def test_gradient_agrees_with_differences():
     """Directional derivative of a smooth loss: central differences at step s are off by s^2 of the third derivative and by
     the loss's fp32 rounding over s; 1e-3 relative covers both at s = 1e-2."""
