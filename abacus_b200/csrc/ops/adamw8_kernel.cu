@@ -20,7 +20,9 @@
 //
 // Bound by memory: 16 bytes an element with fp32 gradients (weight read and
 // written, gradient read, two one-byte moments read and written) and 8 bytes a
-// block for each scale. One warp takes a block of 256 elements, which makes
+// block for each scale; 407 million parameters in 121 tensors take 1.18 ms,
+// 5.5 TB/s (the measured copy rate is 6.56), with three quarters of the issue
+// slots taken. One warp takes a block of 256 elements, which makes
 // the scale one warp-wide integer maximum (magnitudes of floats order as
 // their bits), and each lane two groups of 4 elements, so all loads and stores
 // of a warp are whole lines.
@@ -66,8 +68,8 @@ __device__ __forceinline__ float half_over_root(float x) {
 // The root of x rounded to nearest, from an approximation s of it: one step of Heron's method, s + (x - s^2) / (2 s) with
 // the difference exact, is off by the square of s's error, so its rounding is the root's but for one number in a million.
 // The moment that is kept needs that (which of two codes a number gets depends on its last bit where it meets its
-// threshold, and one code is an eighth of it), the weight's update does not. The correctly rounded library root does the
-// same and made the kernel 11 to 100 % slower with the registers it takes.
+// threshold, and one code is an eighth of it), the weight's update does not. The library's correctly rounded root took
+// 586 to 1077 us for 200 million elements, by the blocks an SM that its registers leave; this one 580.
 __device__ __forceinline__ float polished(float s, float x) { return fmaf(fmaf(-s, s, x), half_over_root(x), s); }
 
 // The e4m3 code of x, rounded stochastically by 16 random bits; |x| < 256. Times 2^-120, e4m3's smallest normal number

@@ -200,7 +200,7 @@ def main():
             "seq_len": sl,
             "layers": args.layers,
             "parallelism": parallelism,
-            "dtype": args.precision if args.impl == "abacus" else "fp32",
+            "dtype": (args.precision if args.impl == "abacus" else "fp32") + (", bf16 experts" if args.expert_dtype == "bf16" else ""),
             "max_mem_gib": round(float(mem), 1),
             "clocks": clocks,
             "data": "synthetic",

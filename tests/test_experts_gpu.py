@@ -337,6 +337,14 @@ def test_plan(tokens, choices, n_experts):
         assert torch.equal(a.cpu(), b)
 
 
+def test_plan_of_more_assignments_than_parts_of_the_smallest_size():
+    """Above 2^20 assignments a block takes more of them."""
+    g = torch.Generator().manual_seed(9)
+    indices = torch.randint(-1, 6, (700001, 2), generator=g)
+    for a, b in zip(experts.expert_plan(indices.cuda(), 5), experts.expert_plan(indices, 5)):
+        assert torch.equal(a.cpu(), b)
+
+
 @pytest.mark.parametrize("indices", ["all to one", "all dropped", "int32"])
 def test_plan_of_one_sided_routings(indices):
     idx = {"all to one": torch.full((5000, 2), 3), "all dropped": torch.full((5000, 2), -1),
