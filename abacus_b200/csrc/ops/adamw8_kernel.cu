@@ -77,12 +77,12 @@ __device__ __forceinline__ float polished(float s, float x) { return fmaf(fmaf(-
 // bits of the float, and adding the random bits below them before they are cut rounds up with the right probability and
 // carries into the exponent where it should. (fp32 keeps 20 bits below the grid; what it drops in a subnormal product is
 // rounded to nearest first.)
-__device__ __forceinline__ uint32_t to_code(float x, unsigned noise16) {
-  const uint32_t t = __float_as_uint(x * 0x1p-120f) + (noise16 << 4);
+__device__ __forceinline__ uint32_t to_code(float x, unsigned noise16) {  // x times 2^-120
+  const uint32_t t = __float_as_uint(x) + (noise16 << 4);
   return (t << 4) | (t & 0x80000000u);  // in the top byte
 }
 __device__ __forceinline__ uint32_t to_code_positive(float x, unsigned noise16) {
-  return (__float_as_uint(x * 0x1p-120f) + (noise16 << 4)) >> 20;  // in the lowest byte
+  return (__float_as_uint(x) + (noise16 << 4)) >> 20;  // in the lowest byte
 }
 __device__ __forceinline__ uint32_t top_bytes(const uint32_t (&x)[4]) {
   return __byte_perm(__byte_perm(x[0], x[1], 0x0073), __byte_perm(x[2], x[3], 0x0073), 0x5410);
@@ -191,8 +191,10 @@ __global__ void __launch_bounds__(kAdam8Warps * 32, 6) adamw8_kernel(const __gri
   // Biased exponents of the scales; 1 (2^-126) is the smallest normal one.
   const int me = max(static_cast<int>(m_top >> 23) - 7, 1);
   const int ue = max(static_cast<int>(u_top >> 23) - 7, 1);
-  const float m_inv = __uint_as_float(static_cast<unsigned>(254 - me) << 23);
-  const float u_inv = __uint_as_float(static_cast<unsigned>(254 - ue) << 23);
+  // 1 / scale, times 2^-120 at once while that is a normal number (moments below 2^14).
+  const bool usual = max(me, ue) <= 133;
+  const float m_inv = __uint_as_float(static_cast<unsigned>(254 - me - (usual ? 120 : 0)) << 23);
+  const float u_inv = __uint_as_float(static_cast<unsigned>(254 - ue - (usual ? 120 : 0)) << 23);
   if (lane == 0) {
     t.m_scale[lo][block] = __uint_as_float(static_cast<unsigned>(me) << 23);
     t.u_scale[lo][block] = __uint_as_float(static_cast<unsigned>(ue) << 23);
@@ -201,11 +203,20 @@ __global__ void __launch_bounds__(kAdam8Warps * 32, 6) adamw8_kernel(const __gri
   for (int h = 0; h < 2; ++h) {
     const int i = h * 128 + lane * 4;
     uint32_t mq[4], uq[4];
+    if (usual) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned noise = mix(static_cast<unsigned>(begin + i + e), s.step_mix);
-      mq[e] = to_code(m[h][e] * m_inv, noise & 0xffffu);
-      uq[e] = max(to_code_positive(u[h][e] * u_inv, noise >> 16), min(__float_as_uint(u[h][e]), 1u));
+      for (int e = 0; e < 4; ++e) {
+        const unsigned noise = mix(static_cast<unsigned>(begin + i + e), s.step_mix);
+        mq[e] = to_code(m[h][e] * m_inv, noise & 0xffffu);
+        uq[e] = max(to_code_positive(u[h][e] * u_inv, noise >> 16), min(__float_as_uint(u[h][e]), 1u));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned noise = mix(static_cast<unsigned>(begin + i + e), s.step_mix);
+        mq[e] = to_code(m[h][e] * m_inv * 0x1p-120f, noise & 0xffffu);
+        uq[e] = max(to_code_positive(u[h][e] * u_inv * 0x1p-120f, noise >> 16), min(__float_as_uint(u[h][e]), 1u));
+      }
     }
     uint32_t m_codes = top_bytes(mq), u_codes = low_bytes(uq);
     if (spoilt) {

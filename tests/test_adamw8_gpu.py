@@ -117,3 +117,20 @@ def test_codes_are_the_cpu_formulation_s_over_many_elements():
         for which in (2, 4):
             assert (gpu[which][0].cpu().float() != cpu[which][0].float()).sum() <= 1
     torch.testing.assert_close(gpu[0][0].cpu(), cpu[0][0], rtol=1e-6, atol=1e-5)
+
+
+@pytest.mark.parametrize("size", [1e-18, 1e-6, 1e5, 1e15])
+def test_gradients_of_any_size(size):
+    """Scales from 2^-68 to 2^43, on both sides of 2^14, where the kernel takes the scaling in one product or in two."""
+    g = torch.Generator().manual_seed(13)
+    n = 20000
+    tensors = [(torch.randn(n, generator=g), torch.randn(n, generator=g) * size, adamw8.fresh_state(n, "cpu"))]
+    gpu, cpu = _lists(tensors, "cuda"), _lists(tensors, "cpu")
+    for step in range(1, 4):
+        adamw8.step_(*gpu, lr=1e-3, step=step)
+        adamw8.step_(*cpu, lr=1e-3, step=step)
+        for which in (2, 4):
+            assert (gpu[which][0].cpu().float() != cpu[which][0].float()).sum() <= 1
+        for which in (3, 5):
+            assert torch.equal(gpu[which][0].cpu(), cpu[which][0])
+    torch.testing.assert_close(gpu[0][0].cpu(), cpu[0][0], rtol=1e-6, atol=1e-5)
