@@ -224,11 +224,12 @@ class AdamW:
             if saved is None:
                 continue
             if self.state_bits == 8:
-                state = self.state[id(param)] = self._fresh_state(0, param)
-                state["step"] = int(saved["step"])
+                entry = self._fresh_state(0, param)
+                entry["step"] = int(saved["step"])
                 m, v = (saved[key].to(device=param.device, dtype=torch.float32) for key in ("exp_avg", "exp_avg_sq"))
-                state["exp_avg"], state["exp_avg_scale"] = adamw8.quantize(m)
-                state["exp_rms"], state["exp_rms_scale"] = adamw8.quantize(v.sqrt(), positive=True)
+                entry["exp_avg"], entry["exp_avg_scale"] = adamw8.quantize(m)
+                entry["exp_rms"], entry["exp_rms_scale"] = adamw8.quantize(v.sqrt(), positive=True)
+                self.state[id(param)] = entry
                 continue
             self.state[id(param)] = {
                 "step": int(saved["step"]),
