@@ -126,7 +126,7 @@ class AdamW:
     # ------------------------------------------------------------ update
     @torch.no_grad()
     def step(self) -> None:
-        groups: dict[tuple, list] = {}
+        items = []  # every refusal comes before the first count or weight changes
         for param in self.params:
             span = self._span(param)
             if span is _NOT_OWNED:
@@ -146,6 +146,11 @@ class AdamW:
             if self.state_bits == 32 and state["exp_avg"].shape != weight.shape:  # flat moments of a whole parameter
                 state["exp_avg"] = state["exp_avg"].view(weight.shape)
                 state["exp_avg_sq"] = state["exp_avg_sq"].view(weight.shape)
+            if self.state_bits == 8 and state["exp_avg"].numel() != weight.numel():
+                raise ValueError(f"AdamW: {state['exp_avg'].numel()} moments of a parameter that steps {weight.numel()} weights")
+            items.append((weight, grad, state))
+        groups: dict[tuple, list] = {}
+        for weight, grad, state in items:
             state["step"] += 1
             key = (weight.device, state["step"], weight.is_cuda and weight.dtype == torch.float32)
             groups.setdefault(key, []).append((weight, grad, state))
