@@ -204,7 +204,8 @@ class AdamW:
         torch._foreach_addcdiv_(weights, m, denom, value=-(self.lr / correction1))
 
     # ------------------------------------------------------------ checkpoints
-    def moments(self, state: dict) -> dict[str, torch.Tensor]:
+    @staticmethod
+    def moments(state: dict) -> dict[str, torch.Tensor]:
         """``{"exp_avg", "exp_avg_sq"}`` of a parameter's state in 32 bits."""
         if "exp_rms" not in state:
             return {key: state[key] for key in ("exp_avg", "exp_avg_sq")}

@@ -24,6 +24,7 @@ from __future__ import annotations
 import torch
 import torch.distributed as dist
 
+from abacus_b200.optim.adamw import AdamW
 from abacus_b200.parallel import mesh
 
 # name suffix -> (mesh dim, concat axis) of sharded parameters
@@ -103,7 +104,7 @@ def full_optimizer_state(model, optimizer, parallel=None) -> dict[str, dict]:
         dist.all_reduce(t, op=dist.ReduceOp.MAX, group=parallel.group)
         step = int(t.item())
     moments = {}
-    local = {pid: optimizer.moments(st) for pid, st in states.items() if st is not None}
+    local = {pid: AdamW.moments(st) for pid, st in states.items() if st is not None}
     for key in ("exp_avg", "exp_avg_sq"):
         pieces = {pid: st[key] for pid, st in local.items()}
         if owned is not None:
