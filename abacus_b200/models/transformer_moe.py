@@ -51,8 +51,8 @@ class TransformerBlockMoe(torch.nn.Module):
             hidden_dim=hidden_dim, bias_update_speed=bias_update_speed, route_scale=route_scale, router=router,
             capacity_factor=capacity_factor, aux_loss_coeff=aux_loss_coeff,
         )
-        if expert_parallel and ragged:
-            raise ValueError("ragged experts do not combine with expert parallel")
+        if expert_parallel and (ragged or expert_dtype is not None):
+            raise ValueError("ragged experts and their type do not combine with expert parallel")
         if expert_parallel:
             self.moe = MoEExpertParallel(dim, n_experts, top_k, data_parallel=expert_data_parallel, **kwargs)
         else:
