@@ -44,7 +44,7 @@ import bench  # noqa: E402  (timing, clocks and process-group helpers)
 VOCAB = 50304
 
 
-def parse_args():
+def parse_args(argv=None):
     p = argparse.ArgumentParser()
     p.add_argument("--config", choices=("tp", "moe", "cppp"), required=True)
     p.add_argument("--impl", choices=("abacus", "reference"), default="abacus")
@@ -58,7 +58,13 @@ def parse_args():
     p.add_argument("--expert-dtype", choices=("fp32", "bf16"), default="fp32", help="moe with --ragged: type of the experts' products")
     p.add_argument("--state-bits", type=int, choices=(8, 32), default=32, help="moe: AdamW's moments")
     p.add_argument("--layers", type=int, default=None, help="override the layer count (smoke runs only)")
-    return p.parse_args()
+    args = p.parse_args(argv)
+    # A flag that nothing would read is refused, so that the line printed says what ran.
+    if (args.ragged or args.expert_dtype != "fp32" or args.state_bits != 32) and (args.config != "moe" or args.impl != "abacus"):
+        p.error("--ragged, --expert-dtype and --state-bits belong to --config moe of this framework")
+    if args.expert_dtype != "fp32" and not args.ragged:
+        p.error("--expert-dtype needs --ragged")
+    return args
 
 
 DEFAULTS = {"tp": (16, 2048), "moe": (64, 1024), "cppp": (8, 16384)}
