@@ -348,7 +348,8 @@ void with_pack(const torch::Tensor& t, int n, F&& f) {
 }
 
 void check_rows(const torch::Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && t.stride(1) == 1 &&
+  // (The stride of a single column says nothing: a transposed row has a stride of its length there.)
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) &&
                   (t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16),
               name, " must be a 2-D fp32 or bf16 CUDA tensor with unit inner stride");
 }
