@@ -10,6 +10,10 @@ namespace ragged {
 
 constexpr int kMaxExperts = 256;
 
+// Rows whose products a weight gradient with one plane sums in one accumulator; with more rows in an expert it needs the
+// workspace of Params::partial.
+constexpr int kRunRows = 1 << 14;
+
 enum Epilogue : int { kStore = 0, kSwiGLU = 1, kSwiGLUBwd = 2 };
 
 // What a launch computes, over sorted rows r of expert e = [offsets[e], offsets[e + 1]):
@@ -38,6 +42,7 @@ struct alignas(64) Params {
   long long ld_in;     // of in
   long long plane;     // distance of the planes of an operand that is written
   int wide;            // rows of a plain result can move in 16-byte units
+  float* partial;      // weights with one plane and more than kRunRows rows: partial_floats() of each CTA
   int* status;
 };
 
@@ -52,6 +57,9 @@ struct Shape {
 // Tile of a shape.
 constexpr int tile_rows(bool pair) { return pair ? 256 : 128; }
 constexpr int tile_cols(bool pair) { return pair ? 256 : 128; }
+
+// Sums of one CTA's part of a tile, 128 rows by a tile's columns.
+constexpr long long partial_floats(bool pair) { return 128ll * tile_cols(pair); }
 
 // Launches with at most `units` output tiles to do; cudaErrorInvalidValue for a combination that is not built.
 cudaError_t launch(const Params& p, const Shape& s, long long units, int sms, cudaStream_t stream);

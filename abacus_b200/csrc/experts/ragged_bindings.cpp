@@ -305,6 +305,11 @@ void weights(torch::Tensor x, std::vector<torch::Tensor> dy, torch::Tensor offse
   p.n_tiles = tiles_of(n, tile_cols(shape.pair));
   p.ld[0] = n;
   p.wide = wide({dw[0], dw.back()}, n);
+  torch::Tensor partial;
+  if (planes == 1 && s > kRunRows) {
+    partial = torch::empty({sms_of(x), partial_floats(shape.pair)}, x.options().dtype(torch::kFloat32));
+    p.partial = partial.data_ptr<float>();
+  }
   run(p, shape, x);
 }
 

@@ -9,11 +9,16 @@
 // three of the 3xTF32 kernels do, with no conversion inside this kernel: the
 // planes are laid out by one pass over each operand before it.
 //
-// Accumulation: the tensor core adds in fp32 but truncates. With one plane a
-// tile's whole sum stays in tensor memory (the outputs are rounded to 8 bits).
-// With several planes each 64 elements of the contraction go into a fresh
-// accumulator, small products first, and the epilogue warps add it to their
-// registers rounding to nearest, so the error is that of an fp32 sum.
+// Accumulation: the tensor core adds in fp32 but truncates. With several planes
+// each 64 elements of the contraction go into a fresh accumulator, small products
+// first, and the epilogue warps add it to their registers rounding to nearest, so
+// the error is that of an fp32 sum. With one plane the outputs are rounded to 8
+// bits, and a tile's whole sum stays in tensor memory; but `weights`, whose
+// contraction is as long as an expert has rows, starts a fresh accumulator every
+// 2^14 rows, and the epilogue warps add the runs up through a workspace, rounding
+// to nearest. (In one accumulator sums of 2^20 positive numbers came out 0.7 %
+// low, of 2^17 ones 0.025 %, of 2^14 0.004 %. Sums in registers need 128 of them a
+// thread and with that a register split; they cost shorter calls 1 to 2 %.)
 //
 // Roles of a CTA (384 threads): warp 0 loads tiles by TMA, warp 1 issues the
 // MMAs, warps 2 and 3 clear the rows of a tile that belong to the next expert (the
@@ -45,6 +50,9 @@ constexpr int kDepth = 64;        // contraction elements of a stage: 128 bytes 
 constexpr int kThreads = 384;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
 constexpr int kStageOutBytes = 32 * 128;  // an epilogue warp's 32 rows of 128 bytes
+
+// Stages of `weights` with one plane whose products share an accumulator.
+constexpr int kRun = kRunRows / kDepth;
 
 constexpr bool split_registers(int planes, Epilogue epi) { return planes > 1 || epi == kSwiGLUBwd; }
 
@@ -544,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
         const Tile t = tile_at(unit, e);
         const uint32_t idesc = t.narrow ? idesc_narrow : idesc_wide;
         for (int step = 0; step < t.steps; ++step, at.next()) {
-          const bool first = PLANES > 1 || step == 0;
+          const bool first = PLANES > 1 || (WEIGHTS ? step % kRun == 0 : step == 0);
           const int buf = acc.stage;
           if (first && acc.wrapped && !wait_bar(&accum_empty[buf], acc.parity ^ 1u, p.status, kStatusTimeoutAccum)) {
             ok = false;
@@ -578,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
           }
           product(0, 0, PLANES == 1 && first);
           commit(&empty_bar[s]);
-          if (PLANES > 1 || step + 1 == t.steps) {
+          if (PLANES > 1 || step + 1 == t.steps || (WEIGHTS && (step + 1) % kRun == 0)) {
             commit(&accum_full[buf]);
             acc.next();
           }
@@ -654,6 +662,14 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       }
       float acc[PLANES > 1 ? kCols : 1];
       int buf = 0;
+      auto release = [&] {  // the accumulator was read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster(leader_addr(&accum_empty[buf]));
+          else mbar_arrive(&accum_empty[buf]);
+        }
+      };
       if constexpr (PLANES > 1) {
 #pragma unroll
         for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
@@ -670,12 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 32; ++i) acc[c + i] += __uint_as_float(v[i]);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if (PAIR) mbar_arrive_cluster(leader_addr(&accum_empty[buf]));
-            else mbar_arrive(&accum_empty[buf]);
-          }
+          release();
         }
       } else if (t.steps > 0) {
         buf = at.stage;
@@ -707,11 +718,44 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       };
       if constexpr (EPI == kStore) {
         Out* out = static_cast<Out*>(p.out[t.output]) + first * p.ld[0];
+        if constexpr (PLANES == 1 && WEIGHTS) {
+          // All runs but the last end in the workspace, where a thread finds its own numbers again.
+          float* partial = p.partial + (static_cast<long long>(blockIdx.x) * kCols * kEpiWarps + (warp - kEpiWarp0)) * 32 + lane;
+          for (int step = kRun; step < t.steps && ok; step += kRun) {
 #pragma unroll 1
-        for (int c = 0; c < kCols; c += 32) {
-          float v[32];
-          columns(c, v);
-          Rows32<Out>::store(mine, lane, out, p.ld[0], rows, t.n0 + half * kCols + c, p.n, p.wide, v);
+            for (int c = 0; c < kCols; c += 32) {
+              float v[32];
+              columns(c, v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                float* sum = partial + (c + i) * kEpiWarps * 32;
+                *sum = step == kRun ? v[i] : *sum + v[i];
+              }
+            }
+            release();
+            at.next();
+            buf = at.stage;
+            ok = wait_bar_warp(&accum_full[buf], at.parity, p.status, kStatusTimeoutAccum);
+            tc_fence_after();
+          }
+          if (!ok) break;
+#pragma unroll 1
+          for (int c = 0; c < kCols; c += 32) {
+            float v[32];
+            columns(c, v);
+            if (t.steps > kRun) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] += partial[(c + i) * kEpiWarps * 32];
+            }
+            Rows32<Out>::store(mine, lane, out, p.ld[0], rows, t.n0 + half * kCols + c, p.n, p.wide, v);
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < kCols; c += 32) {
+            float v[32];
+            columns(c, v);
+            Rows32<Out>::store(mine, lane, out, p.ld[0], rows, t.n0 + half * kCols + c, p.n, p.wide, v);
+          }
         }
       } else if constexpr (EPI == kSwiGLU) {
 #pragma unroll 1
@@ -784,12 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
         }
       }
       if (PLANES == 1 && t.steps > 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (PAIR) mbar_arrive_cluster(leader_addr(&accum_empty[buf]));
-          else mbar_arrive(&accum_empty[buf]);
-        }
+        release();
         at.next();
       }
     }
