@@ -9,6 +9,7 @@
 #include <cuda_bf16.h>
 #include <cstdint>
 #include "few.h"
+#include "sigmoid.cuh"
 
 namespace abacus {
 namespace ragged {
@@ -280,13 +281,13 @@ __global__ void __launch_bounds__(kThreads) outer_kernel(const FewParams p) {
 
 __global__ void __launch_bounds__(kThreads) few_swiglu_kernel(const float* g, const float* u, float* h, long long n) {
   for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads)
-    h[i] = g[i] * __fdividef(1.f, 1.f + __expf(-g[i])) * u[i];
+    h[i] = g[i] * sigmoid<24>(g[i]) * u[i];
 }
 
 __global__ void __launch_bounds__(kThreads) few_swiglu_bwd_kernel(const float* dh, const float* g, const float* u, float* dg,
                                                                   float* du, long long n) {
   for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * kThreads) {
-    const float x = g[i], sig = __fdividef(1.f, 1.f + __expf(-x)), through = dh[i] * sig;
+    const float x = g[i], sig = sigmoid<24>(x), through = dh[i] * sig;
     dg[i] = through * u[i] * (1.f + x * (1.f - sig));
     du[i] = through * x;
   }

@@ -41,6 +41,7 @@
 #include "../common/host.h"
 #include "../common/sm100.cuh"
 #include "ragged.h"
+#include "sigmoid.cuh"
 #include "split.cuh"
 
 namespace abacus {
@@ -320,10 +321,6 @@ __device__ __forceinline__ void store_operand(uint8_t* staging, int lane, __nv_b
     }
   }
 }
-
-// Within 2^-21: far inside the rounding of what it is multiplied into, and a quarter of the instructions of a correctly
-// rounded quotient.
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
 struct Tile {
   int expert;     // == experts: rows that nobody owns
@@ -781,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
           store_kept(mine, lane, static_cast<float*>(p.out[0]) + first * p.ld[0], p.ld[0], rows, col, p.n, gate);
           store_kept(mine, lane, static_cast<float*>(p.out[1]) + first * p.ld[1], p.ld[1], rows, col, p.n, up);
 #pragma unroll
-          for (int i = 0; i < kSpanCols; ++i) up[i] *= gate[i] * sigmoid(gate[i]);
+          for (int i = 0; i < kSpanCols; ++i) up[i] *= gate[i] * sigmoid<PLANES == 1 ? 8 : 24>(gate[i]);
           store_operand<PLANES>(mine, lane, static_cast<__nv_bfloat16*>(p.out[2]) + first * p.ld[2], p.plane, p.ld[2], rows,
                                 col, p.n, up);
         }
@@ -815,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float sig = sigmoid(g[j]);
+              const float sig = sigmoid<8>(g[j]);
               const float through = d[j] * sig;
               d[j] = through * u[j] * (1.f + g[j] * (1.f - sig));
               g[j] *= through;

@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 #include "../common/sm100.cuh"
 #include "ragged.h"
+#include "sigmoid.cuh"
 #include "split.cuh"
 
 namespace abacus {
@@ -73,7 +74,7 @@ __global__ void __launch_bounds__(256) swiglu_bwd_kernel(const SwiGLUBwdParams p
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float sig = __fdividef(1.f, 1.f + __expf(-g[j]));
+      const float sig = sigmoid<24>(g[j]);
       const float through = d[j] * sig;
       d[j] = through * u[j] * (1.f + g[j] * (1.f - sig));
       g[j] *= through;
