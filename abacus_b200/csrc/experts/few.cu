@@ -9,6 +9,7 @@
 #include <cuda_bf16.h>
 #include <cstdint>
 #include "few.h"
+#include "offsets.cuh"
 #include "sigmoid.cuh"
 
 namespace abacus {
@@ -140,6 +141,8 @@ __global__ void __launch_bounds__(kThreads) few_kernel(const FewParams p) {
   __shared__ __align__(16) float smem[kFloats];
   const int e = blockIdx.y, col0 = blockIdx.x * C;
   if (e == p.experts) {
+    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x < 32)
+      check_offsets(p.offsets, p.experts, p.rows, threadIdx.x, p.status);
     if (blockIdx.z == 0) zero_columns<TO>(p, col0, C);
     return;
   }
@@ -218,6 +221,8 @@ __global__ void __launch_bounds__(kThreads) dot_kernel(const FewParams p) {
   constexpr int C = kWarps * kDots;
   const int e = blockIdx.y, col0 = blockIdx.x * C;
   if (e == p.experts) {
+    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x < 32)
+      check_offsets(p.offsets, p.experts, p.rows, threadIdx.x, p.status);
     if (blockIdx.z == 0) zero_columns<TO>(p, col0, C);
     return;
   }
@@ -237,6 +242,8 @@ constexpr int kOutRows = 8;
 template <class TA, class TB, class TO, bool WIDE>
 __global__ void __launch_bounds__(kThreads) outer_kernel(const FewParams p) {
   const int e = blockIdx.z, lane = threadIdx.x % 32;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && e == 0 && threadIdx.x < 32)
+    check_offsets(p.offsets, p.experts, p.rows, lane, p.status);
   // Four columns side by side where they can be stored at once, else 32 apart.
   const int n0 = blockIdx.x * 128 + lane * (WIDE ? 4 : 1), m0 = (blockIdx.y * kWarps + threadIdx.x / 32) * kOutRows;
   constexpr int kApart = WIDE ? 1 : 32;

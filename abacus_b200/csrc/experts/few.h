@@ -24,6 +24,7 @@ struct FewParams {
   const int* offsets;
   int experts, rows;
   int k, n, m;
+  int* status;
 };
 // out[r] = a[r] B[e], B (k, n).      out[r] = a[r] B[e]^T + add[r], B (n, k).      out[e] = sum_r a[r]^T b[r], (m, n).
 cudaError_t launch_few(const FewParams& p, cudaStream_t stream);

@@ -120,6 +120,7 @@ ragged::FewParams few_params(const Tensor& a, const Tensor& b, const Tensor& off
   p.offsets = offsets.data_ptr<int>();
   p.experts = static_cast<int>(offsets.numel() - 1);
   p.rows = static_cast<int>(a.size(0));
+  p.status = host::status_ptr(static_cast<int>(a.get_device()));
   return p;
 }
 

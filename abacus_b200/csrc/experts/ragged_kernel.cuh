@@ -40,6 +40,7 @@
 #include <type_traits>
 #include "../common/host.h"
 #include "../common/sm100.cuh"
+#include "offsets.cuh"
 #include "ragged.h"
 #include "sigmoid.cuh"
 #include "split.cuh"
@@ -383,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
   }
   // Offsets are the caller's device data: whatever they hold, every range used is inside [0, rows].
   auto offset_at = [&](int e) { return e == 0 ? 0 : min(max(p.offsets[e], 0), p.rows); };
+  if (warp == 2 && blockIdx.x == 0) check_offsets(p.offsets, p.experts, p.rows, lane, p.status);
   if (!WEIGHTS && warp == 3) {
     // Row tiles before each expert; the rows after the last one's are expert number `experts`.
     int carry = 0;
@@ -392,7 +394,6 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_kernel(const __grid_consta
       if (e <= p.experts) {
         const int begin = offset_at(e), end = e == p.experts ? p.rows : offset_at(e + 1);
         tiles = (max(end - begin, 0) + kTileM - 1) / kTileM;
-        if (end < begin && blockIdx.x == 0) atomicCAS(p.status, kStatusOk, kStatusBadArgs);
       }
       int sum = tiles;
 #pragma unroll

@@ -98,8 +98,10 @@ def _fp32_planes() -> int:
     return 3 if precision.passes() == 3 else 2
 
 
-def _cpu_spans(offsets: torch.Tensor) -> list[tuple[int, int]]:
+def _cpu_spans(offsets: torch.Tensor, rows: int) -> list[tuple[int, int]]:
     ends = offsets.tolist()
+    if ends[0] != 0 or ends[-1] > rows or any(b < a for a, b in zip(ends[:-1], ends[1:])):
+        raise ValueError(f"offsets must start at 0, not decrease and end within the {rows} rows, got {ends}")
     return list(zip(ends[:-1], ends[1:]))
 
 
@@ -121,14 +123,15 @@ def _check_products(x: torch.Tensor, mats: dict[str, torch.Tensor], shapes: dict
 def ragged_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     """``y[r] = x[r] @ w[e]`` for the rows ``offsets[e] <= r < offsets[e + 1]`` of ``x`` (S, D), with ``w`` (E, D, N).
 
-    ``offsets`` starts at 0 and does not decrease. Rows at or after ``offsets[E]`` belong to nobody: their ``y`` and
+    ``offsets`` starts at 0, does not decrease and ends within the rows: CPU tensors raise if not; on the GPU, where nobody
+    waits for them, the device status says so (``_ext.check_status``), and the results are in bounds but say nothing. Rows at or after ``offsets[E]`` belong to nobody: their ``y`` and
     gradient are zeros and they add nothing to ``w``'s gradient, whatever they hold."""
     if x.is_cuda:
         return ext().ragged_matmul(x, w, offsets, _fp32_planes())
     if w.ndim != 3:
         raise ValueError(f"w must be (experts, in, out), got {tuple(w.shape)}")
     _check_products(x, {"w": w}, {"w": (x.shape[-1], w.shape[2])}, offsets)
-    parts = [x[a:b] @ w[e] for e, (a, b) in enumerate(_cpu_spans(offsets))]
+    parts = [x[a:b] @ w[e] for e, (a, b) in enumerate(_cpu_spans(offsets, x.shape[0]))]
     return torch.cat([*parts, x.new_zeros(x.shape[0] - int(offsets[-1]), w.shape[2])])
 
 
@@ -143,5 +146,5 @@ def ragged_swiglu_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     _check_products(x, {"w_gate": w_gate, "w_up": w_up, "w_down": w_down},
                     {"w_gate": (d, hidden), "w_up": (d, hidden), "w_down": (hidden, w_down.shape[2])}, offsets)
     parts = [(torch.nn.functional.silu(x[a:b] @ w_gate[e]) * (x[a:b] @ w_up[e])) @ w_down[e]
-             for e, (a, b) in enumerate(_cpu_spans(offsets))]
+             for e, (a, b) in enumerate(_cpu_spans(offsets, x.shape[0]))]
     return torch.cat([*parts, x.new_zeros(x.shape[0] - int(offsets[-1]), w_down.shape[2])])
