@@ -8,6 +8,7 @@
 // again from L2. 32 experts of 2048 x 2048 in fp32 take 93 us with a row each (5.8 TB/s) and 131 us with four.
 #include <cuda_bf16.h>
 #include <cstdint>
+#include <type_traits>
 #include "few.h"
 #include "offsets.cuh"
 #include "sigmoid.cuh"
@@ -308,27 +309,25 @@ bool wide_b(const FewParams& p, int row_length) {
   return aligned(p.b, 16) && row_length % unit == 0 && p.ld_b % unit == 0 && p.stride_b % unit == 0;
 }
 
-// f(zero of the rows' type, of the matrices', of the result's) for the combinations in use.
-template <class F>
+// f(zero of a's type, of b's, of the result's) for the combinations that a product is called with: bits 4, 2 and 1 of a
+// combination say which of the three are bf16.
+template <int... USED, class F>
 cudaError_t with_types(const FewParams& p, F&& f) {
-  using H = __nv_bfloat16;
   const int which = (p.a_bf16 ? 4 : 0) | (p.b_bf16 ? 2 : 0) | (p.out_bf16 ? 1 : 0);
-  switch (which) {
-    case 0: f(float{}, float{}, float{}); break;
-    case 3: f(float{}, H{}, H{}); break;
-    case 2: f(float{}, H{}, float{}); break;
-    case 5: f(H{}, float{}, H{}); break;
-    case 6: f(H{}, H{}, float{}); break;
-    case 7: f(H{}, H{}, H{}); break;
-    default: return cudaErrorInvalidValue;
-  }
-  return cudaGetLastError();
+  auto call = [&](auto used) {
+    constexpr int kUsed = decltype(used)::value;
+    if (which != kUsed) return false;
+    f(std::conditional_t<(kUsed & 4) != 0, __nv_bfloat16, float>{}, std::conditional_t<(kUsed & 2) != 0, __nv_bfloat16, float>{},
+      std::conditional_t<(kUsed & 1) != 0, __nv_bfloat16, float>{});
+    return true;
+  };
+  return (call(std::integral_constant<int, USED>{}) || ...) ? cudaGetLastError() : cudaErrorInvalidValue;
 }
 
 // Blocks that share an expert's rows, so that an expert which has most of them is not left to one block a strip (256 rows,
 // all of one of 32 experts of 2048 x 2816 in fp32: 243 us against 787); those without rows leave at once (evenly spread
 // rows: 234 us against 250 for 8 rows of each of 32 experts of 2048 x 2048).
-unsigned shares_of(const FewParams& p) { return p.rows >= 256 ? 8 : (p.rows + 31) / 32; }
+unsigned shares_of(const FewParams& p) { return (p.rows + 31) / 32; }
 
 unsigned blocks_of(long long n) {
   const long long b = (n + kThreads - 1) / kThreads;
@@ -341,7 +340,7 @@ cudaError_t launch_few(const FewParams& p, cudaStream_t stream) {
   const bool wide = wide_b(p, p.n);
   const int cols = 8 * (p.b_bf16 ? 8 : 4);
   const dim3 grid((p.n + cols - 1) / cols, p.experts + 1, shares_of(p));
-  return with_types(p, [&](auto a, auto b, auto o) {
+  return with_types<0, 3, 6, 7>(p, [&](auto a, auto b, auto o) {
     using A = decltype(a);
     using B = decltype(b);
     using O = decltype(o);
@@ -353,7 +352,7 @@ cudaError_t launch_few(const FewParams& p, cudaStream_t stream) {
 cudaError_t launch_few_transposed(const FewParams& p, cudaStream_t stream) {
   const bool wide = wide_b(p, p.k);
   const dim3 grid((p.n + kWarps * kDots - 1) / (kWarps * kDots), p.experts + 1, shares_of(p));
-  return with_types(p, [&](auto a, auto b, auto o) {
+  return with_types<0, 2, 3, 6, 7>(p, [&](auto a, auto b, auto o) {
     using A = decltype(a);
     using B = decltype(b);
     using O = decltype(o);
@@ -365,7 +364,7 @@ cudaError_t launch_few_transposed(const FewParams& p, cudaStream_t stream) {
 cudaError_t launch_few_weights(const FewParams& p, cudaStream_t stream) {
   const bool wide = p.n % 4 == 0 && aligned(p.out, 16);
   const dim3 grid((p.n + 127) / 128, (p.m + kWarps * kOutRows - 1) / (kWarps * kOutRows), p.experts);
-  return with_types(p, [&](auto a, auto b, auto o) {
+  return with_types<0, 3, 5, 7>(p, [&](auto a, auto b, auto o) {
     using A = decltype(a);
     using B = decltype(b);
     using O = decltype(o);

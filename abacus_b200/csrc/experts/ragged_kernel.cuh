@@ -191,14 +191,6 @@ struct OutTraits<__nv_bfloat16> {
     }
     return u;
   }
-  __device__ static void unpack(uint4 u, float* v) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
 };
 
 // Stores 32 columns of a warp's 32 rows, a row a lane, through the warp's staging rows, so that global accesses run

@@ -28,7 +28,6 @@ from abacus_b200.ops._ext import ext
 
 BLOCK = 256
 _MASK32 = 0xFFFFFFFF
-_MAX_CODE = 448.0  # the largest e4m3 number
 
 
 def fresh_state(numel: int, device) -> dict[str, torch.Tensor]:
