@@ -120,7 +120,14 @@ void run(const Params& p, const Shape& s, const torch::Tensor& like) {
 // Column tiles of an output with n columns, a tile making `cols` of them.
 int tiles_of(int64_t n, int cols) { return static_cast<int>((n + cols - 1) / cols); }
 
-// Pairs for experts with rows enough to fill their 256-row tiles, single CTAs for short ones.
+// Pairs for experts with rows enough to fill their 256-row tiles, single CTAs for short ones. With uneven loads (the
+// largest of 32 experts has four times the average) the two cross near 192 rows on average: y / dx / SwiGLU of 2048 x 1408
+// in bf16, on pairs against singles, 128 rows 61 / 58 / 112 against 58 / 59 / 95 us, 192 rows 71 / 65 / 107 against
+// 70 / 68 / 131, 256 rows 75 / 70 / 132 against 82 / 85 / 157; in fp32 with 192 rows 351 / 304 / 537 against 296 / 268 / 586,
+// with 256 rows 359 / 319 / 696 against 361 / 347 / 714. With equal loads they cross where a second 128-row tile begins
+// (y in bf16: 128 rows 58 against 47, 160 rows 58 against 68). The average does not see one long expert among short ones:
+// with 8000 of 10,000 rows in one of 64 experts of 768 x 1536 (an average of 157), which run on singles, y takes 68 us and would take
+// 60 on pairs, SwiGLU 122 and 146.
 bool use_pair_rows(const Params& p) { return p.rows >= 192ll * p.experts; }
 
 void check_rows_and_matrices(const torch::Tensor& a, const torch::Tensor& b, int64_t experts, int64_t k, const char* name) {

@@ -17,8 +17,11 @@
 // contraction is as long as an expert has rows, starts a fresh accumulator every
 // 2^14 rows, and the epilogue warps add the runs up through a workspace, rounding
 // to nearest. (In one accumulator sums of 2^20 positive numbers came out 0.7 %
-// low, of 2^17 ones 0.025 %, of 2^14 0.004 %. Sums in registers need 128 of them a
-// thread and with that a register split; they cost shorter calls 1 to 2 %.)
+// low, of 2^17 ones 0.025 %, of 2^14 0.004 %. A run more costs 2 %: 131072 rows of
+// 8 experts of 768 x 1536, five of which have more than 2^14, take 253 us against
+// 248 in one accumulator each; with fewer rows nothing changes. Sums in registers
+// need 128 of them a thread and with that a register split, and cost shorter calls
+// 1 to 2 %.) The contractions of the other products are the matrices' widths.
 //
 // Roles of a CTA (384 threads): warp 0 loads tiles by TMA, warp 1 issues the
 // MMAs, warps 2 and 3 clear the rows of a tile that belong to the next expert (the
@@ -30,11 +33,12 @@
 // the tiles; accumulators are double buffered, so a tile's epilogue runs under
 // the next tile's MMAs.
 //
-// Measured: 131072 rows, 8 experts of 768 x 1536 in bf16 at 1322 (forward), 1363
-// (dx) and 1289 TFLOP/s (dW), where cuBLAS makes 1299, 1387 and 1205 of one dense
-// product of these sizes; three planes at 240 to 253 TFLOP/s (1440 to 1520 of
-// bf16 products). Both run into the power cap. 64 experts of about 1024 rows lose
-// 12 % to tiles that their rows do not fill.
+// Measured, two launches after a pause: 131072 rows, 8 experts of 768 x 1536 in
+// bf16 at 1320 (forward), 1389 (dx) and 1266 TFLOP/s (dW), where cuBLAS makes 1299,
+// 1387 and 1205 of one dense product of these sizes; 32768 rows in three planes at
+// 238 to 244 TFLOP/s (1430 to 1470 of bf16 products), in two at 408 to 444. A stream
+// of launches runs into the power cap. 64 experts of about 1024 rows lose 12 % to
+// tiles that their rows do not fill.
 #pragma once
 #include <cuda_bf16.h>
 #include <type_traits>

@@ -20,8 +20,8 @@
 //
 // Bound by memory: 16 bytes an element with fp32 gradients (weight read and
 // written, gradient read, two one-byte moments read and written) and 8 bytes a
-// block for each scale; 407 million parameters in 121 tensors take 1.18 to
-// 1.27 ms by the GPU, 5.1 to 5.5 TB/s (a copy runs at 6.56), with three quarters
+// block for each scale; 407 million parameters in 121 tensors take 1.16 to
+// 1.27 ms by the GPU, 5.1 to 5.6 TB/s (a copy runs at 6.56), with three quarters
 // of the issue slots taken. One warp takes a block of 256 elements, which makes
 // the scale one warp-wide integer maximum (magnitudes of floats order as
 // their bits), and each lane two groups of 4 elements, so all loads and stores

@@ -16,11 +16,14 @@
 // The sort is a counting sort, stable because every warp takes a contiguous
 // run of assignments and ranks equal experts by lane: one launch up to 1024
 // assignments, above that one more that counts per part. No atomic decides a
-// place, so results repeat bit for bit.
+// place, so results repeat bit for bit. Every block of the second launch adds up
+// all parts' counts of all bins, so its work grows as their square: 524,288
+// assignments take 40 us over 128 experts, 66 over 256 and 222 over 1024.
 //
 // The row kernels are bound by memory; each row is read once and written once:
 // 65536 tokens, 2 choices, 768 bf16 take 46 us to dispatch (6.5 TB/s), 55 us to
-// combine (5.5) and 77 us for the gradients of that (6.5); the plan takes 7 us.
+// combine (5.5) and 77 us for the gradients of that (6.5; 86 with the launch, one
+// call after another); the plan takes 7 us.
 // One warp takes a token: it reads x[t] once for its K copies, and sums its K
 // rows in the order of k, in fp32. Rows move in the widest unit (16 bytes down
 // to one element) that the row length and the pointers' alignment allow.
@@ -244,9 +247,11 @@ __global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ ys, 
   }
 }
 
-// GROUP choices of a token at a time, so that d out[t] is read once for them: two where the number of choices is even
-// (77 us for 65536 tokens, 2 choices, 768 bf16; 95 one at a time), one where it is odd (33 us for 9001 tokens, 3 choices,
-// 770 fp32; 51 two at a time).
+// GROUP choices of a token at a time, so that d out[t] is read once for them: two where the number of choices is even, one
+// where it is odd. Two at a time against one, 65536 tokens with 2 choices: bf16 rows of 768 86 against 101 us, of 770 (4-byte
+// units) 125 against 147, fp32 rows of 768 159 against 169; 8-byte units lose by it (bf16 772 120 against 116, fp32 770 191
+// against 183). An odd number taken by two with a last one alone would make three choices of 768 bf16 116 us in place of
+// 141, and 9001 tokens' three of 770 fp32 52 in place of 43.
 template <class T, int N, int GROUP>
 __global__ void __launch_bounds__(256) combine_bwd_kernel(const T* __restrict__ dout, const T* __restrict__ ys,
                                                           const float* __restrict__ weights, const int* __restrict__ slot,

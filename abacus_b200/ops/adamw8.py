@@ -11,9 +11,15 @@ power of two. A step is
 
 in fp32, after which m and u are rounded to 8 bits stochastically, with random
 bits that an integer hash makes of (element number in the tensor, step): the
-same inputs give the same outputs, on the CPU as on the GPU. A second moment
-that is not zero never rounds to zero. A gradient that is infinite or NaN
-spoils its own element (moments NaN, as in 32 bits), not its block.
+same inputs give the same outputs. CPU and GPU take the same random bits; their
+moments agree but for a code in a million or so, their weights to fp32's rounding.
+A second moment that is not zero never rounds to zero. A gradient that is
+infinite or NaN spoils its own element (moments NaN, as in 32 bits), not its block.
+
+The price of one scale for 256 elements: an element whose u is below some 2^-17
+of its block's largest is held at the smallest code, which is larger than what
+it stands for, and moves by that much less than it would with 32-bit moments
+(gradients of 1e-7 among one of 1: 0.0025 in 200 steps of 1e-3 in place of 0.18).
 
 CUDA tensors run on ``csrc/ops/adamw8_kernel.cu`` (one launch for up to 128 tensors);
 CPU tensors run the formulation below.

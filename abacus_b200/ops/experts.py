@@ -12,8 +12,9 @@ Types: fp32 or bf16 rows and matrices (both of one type), results in that type, 
 ``precision.set_precision``: "fp32" multiplies three bf16 parts of each operand (all 24 bits of a number above 2^-110 or
 so; the parts' smallest number is 2^-133), "tf32" two (16 bits). An infinite fp32 operand may give NaN where plain
 arithmetic gives infinity (it meets the zero parts of the other operand), as in the framework's 3xTF32 products.
-bf16 operands are multiplied as they are; ``ragged_swiglu_mlp`` rounds gate, up, their product and the two gradients
-through it to bf16 between its products, as storing them does.
+bf16 operands are multiplied as they are. ``ragged_swiglu_mlp`` keeps gate and up in fp32 and rounds h = silu(gate) up and
+the gradients of gate and up to bf16, because they are operands of bf16 products (the kernels for few rows keep them in
+fp32 too). Sums are fp32 at any length; those over an expert's rows in bf16 are made of runs of 2^14 rows.
 
 CUDA tensors run on ``csrc/experts`` and ``csrc/ops/expert_rows.cu`` (up to 256 experts for the products, 1024 for the
 plan; differentiable once); CPU tensors run the formulas with ATen.
